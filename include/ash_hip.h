@@ -657,7 +657,9 @@ int ash_add_rows(const void* rows, const int64_t* indices, const uint8_t* masks,
 /* -------------------------------------------------------- trilinear queries */
 
 enum { ASH_INTERP_LINEAR = 0, ASH_INTERP_SMOOTH_STEP = 1 };
-enum { ASH_F32 = 0, ASH_F64 = 1 };
+enum { ASH_F32 = 0, ASH_F64 = 1, ASH_BF16 = 2, ASH_F16 = 3, ASH_E4M3 = 4 };
+enum { ASH_ACT_NONE = 0, ASH_ACT_RELU = 1, ASH_ACT_SILU = 2, ASH_ACT_GELU = 3, ASH_ACT_SOFTPLUS = 4,
+       ASH_ACT_SINE = 5 };
 
 /* Operands shared by the three query entry points (ash/src/grid.h:6-82):
  *   embeddings   scalar[B, M, E]   (M = cells per block, E <= 16)
@@ -934,6 +936,98 @@ int ash_marching_cubes_extract(const void* sdfs, const int64_t* grid_indices,
                                uint32_t* edge_slots, int32_t* workspace, int64_t n_vertices,
                                int64_t n_triangles, float* positions, int32_t* triangles,
                                void* stream);
+
+/* ------------------------------------------------------------ layers on features
+ *
+ * What reads the features of a grid or an embedding: dense layers and the
+ * root-mean-square norm, with gradients of first and second order.  The
+ * reference leaves them to torch (ash/mlp.py:43-285); no pybind counterpart.
+ * Values are float32, bfloat16 or float16 (ASH_F32, ASH_BF16, ASH_F16), sums
+ * float32.  Rows are `*_stride` values apart (0: every row is the same one), the
+ * values of a row consecutive; tensors without a stride are contiguous.  No
+ * pointer needs to be aligned to more than a value.
+ *
+ *   output = f(input weight^T * scales + bias) + residual
+ *   f: ASH_ACT_*; with the activation's scale a, SOFTPLUS is log(1 + exp(a z)) / a
+ *   and SINE sin(a z)
+ *
+ * dtype ASH_E4M3: input and weight are 8-bit rows with a float32 scale each, and
+ * bias, residual and output are of out_dtype; otherwise out_dtype is dtype and
+ * the scales are not read.  Up to 65536 features in and out. */
+typedef struct ash_linear_args {
+    const void* input;           /* (rows, in_features) */
+    const void* weight;          /* (out_features, in_features) */
+    const void* bias;            /* (out_features) or NULL */
+    const void* residual;        /* (rows, out_features) or NULL */
+    const float* input_scales;   /* (rows), ASH_E4M3 only */
+    const float* weight_scales;  /* (out_features), ASH_E4M3 only */
+    int64_t rows, in_features, out_features;
+    int64_t input_stride, residual_stride;
+    int32_t dtype, out_dtype, activation;
+    float activation_scale;
+} ash_linear_args;
+
+/* slope: f'(z), for the backward calls, or NULL. */
+int ash_linear_forward(const ash_linear_args* args, void* output, void* slope, void* stream);
+/* grad_input = (grad * slope) weight (+ addend); slope NULL: f'(z) is one.  Reads
+ * weight and the sizes of args. */
+int ash_linear_backward_input(const ash_linear_args* args, const void* grad, const void* slope,
+                              const void* addend, void* grad_input, void* stream);
+/* grad_weight = (grad * slope)^T input and grad_bias = the column sums of grad *
+ * slope, either NULL.  With second_grad, (second_grad * second_slope)^T second_input
+ * is added, and second_has_bias says which of the two the bias' gradient sums.  The
+ * rows are cut into parts whose sums meet in scratch and are joined in their order:
+ * the same numbers on every run.  Reads input and the sizes of args. */
+int64_t ash_linear_backward_weight_scratch_bytes(int64_t rows, int64_t in_features,
+                                                 int64_t out_features, int32_t dtype, int pairs);
+int ash_linear_backward_weight(const ash_linear_args* args, const void* grad, const void* slope,
+                               const void* second_grad, const void* second_slope,
+                               const void* second_input, int64_t second_input_stride,
+                               int second_has_bias, void* grad_weight, void* grad_bias,
+                               void* scratch, int64_t scratch_bytes, void* stream);
+/* Second order.  second_input (or NULL) is the gradient of grad_input, addend (or
+ * NULL) what the gradients of grad_weight (V) and grad_bias (c) give: input V^T + c.  With t = second_input weight^T + addend:
+ *   grad_grad = t f'(z),  curvature = t grad f''(z)   (either NULL)
+ * from which the other gradients follow by the two backward calls. */
+int ash_linear_second(const ash_linear_args* args, const void* grad, const void* second_input,
+                      int64_t second_input_stride, const void* addend, int64_t addend_stride,
+                      void* grad_grad, void* curvature, void* stream);
+
+/* s = input + residual;  y = s (mean s^2 + eps)^-1/2 weight, over rows of 1 to
+ * 16384 values.
+ *
+ * forward: output = y, sum_out = s.  With scales, output is e4m3 (rounded to
+ * nearest) of y / scale, scale = the row's largest |y| / 448; a row of zeros has
+ * the scale 1, one with an infinity or NaN the scale NaN.  normalise 0: y = s.
+ * backward: input is s, grad of y, grad_sum of s (or NULL); output = the
+ * gradient of s (or NULL), weight_out that of weight (or NULL), whose parts meet in
+ * `parts` (ash_norm_backward_scratch_bytes) and are joined in their order.
+ * second: `second` (of the gradient of s) and second_weight (of the weight's),
+ * either NULL; output = what follows for s, grad_out for grad, weight_out for
+ * weight, each or NULL. */
+typedef struct ash_norm_args {
+    const void* input;           /* (rows, cols) */
+    const void* residual;        /* (rows, cols) or NULL; forward only */
+    const void* weight;          /* (cols) or NULL: ones */
+    const void* grad;            /* (rows, cols) */
+    const void* grad_sum;        /* (rows, cols) or NULL */
+    const void* second;          /* (rows, cols) or NULL */
+    const void* second_weight;   /* (cols) or NULL */
+    void* output;                /* (rows, cols) */
+    void* sum_out;               /* (rows, cols) or NULL */
+    void* grad_out;              /* (rows, cols) or NULL */
+    void* weight_out;            /* (cols) or NULL */
+    float* scales;               /* (rows) or NULL */
+    float* parts;
+    int64_t rows, cols, input_stride, residual_stride;
+    int32_t dtype, normalise;
+    float eps;
+} ash_norm_args;
+
+int ash_norm_forward(const ash_norm_args* args, void* stream);
+int64_t ash_norm_backward_scratch_bytes(int64_t rows, int64_t cols);
+int ash_norm_backward(const ash_norm_args* args, void* stream);
+int ash_norm_second(const ash_norm_args* args, void* stream);
 
 #ifdef __cplusplus
 }

@@ -7,20 +7,24 @@ libash_hip.so.
 from .common import DotDict
 from .core import ASHEngine, ASHModule
 from .embedding import HashEmbedding
+from .decoder import FeatureDecoder
 from . import fusion
 from .grid import BoundedSparseDenseGrid, SparseDenseGrid, UnBoundedSparseDenseGrid
 from .grid_nns import enumerate_neighbor_coord_offsets
 from .grid_query import SparseDenseGridQuery, SparseDenseGridQueryBackward, dense_grad
 from .hashmap import HashMap, HashSet
+from .layers import QuantizedRows, linear, rms_norm
 
 __all__ = [
     "ASHEngine",
     "ASHModule",
     "BoundedSparseDenseGrid",
     "DotDict",
+    "FeatureDecoder",
     "HashEmbedding",
     "HashMap",
     "HashSet",
+    "QuantizedRows",
     "SparseDenseGrid",
     "SparseDenseGridQuery",
     "SparseDenseGridQueryBackward",
@@ -28,4 +32,6 @@ __all__ = [
     "dense_grad",
     "enumerate_neighbor_coord_offsets",
     "fusion",
+    "linear",
+    "rms_norm",
 ]

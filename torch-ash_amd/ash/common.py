@@ -56,6 +56,42 @@ class _QueryArgs(ctypes.Structure):
     ]
 
 
+class _LinearArgs(ctypes.Structure):
+    _fields_ = [
+        ("input", _PTR),
+        ("weight", _PTR),
+        ("bias", _PTR),
+        ("residual", _PTR),
+        ("input_scales", _PTR),
+        ("weight_scales", _PTR),
+        ("rows", _I64),
+        ("in_features", _I64),
+        ("out_features", _I64),
+        ("input_stride", _I64),
+        ("residual_stride", _I64),
+        ("dtype", ctypes.c_int32),
+        ("out_dtype", ctypes.c_int32),
+        ("activation", ctypes.c_int32),
+        ("activation_scale", ctypes.c_float),
+    ]
+
+
+class _NormArgs(ctypes.Structure):
+    _fields_ = [
+        (name, _PTR)
+        for name in ("input", "residual", "weight", "grad", "grad_sum", "second", "second_weight",
+                     "output", "sum_out", "grad_out", "weight_out", "scales", "parts")
+    ] + [
+        ("rows", _I64),
+        ("cols", _I64),
+        ("input_stride", _I64),
+        ("residual_stride", _I64),
+        ("dtype", ctypes.c_int32),
+        ("normalise", ctypes.c_int32),
+        ("eps", ctypes.c_float),
+    ]
+
+
 # name -> (restype, argtypes); mirrors include/ash_hip.h
 _SIGNATURES = {
     "ash_last_error": (ctypes.c_char_p, []),
@@ -343,6 +379,23 @@ _SIGNATURES = {
         ctypes.c_int,
         [ctypes.POINTER(_QueryArgs), _PTR, _PTR, _PTR, _PTR, _PTR],
     ),
+    "ash_linear_forward": (ctypes.c_int, [ctypes.POINTER(_LinearArgs), _PTR, _PTR, _PTR]),
+    "ash_linear_backward_input": (ctypes.c_int, [ctypes.POINTER(_LinearArgs)] + [_PTR] * 5),
+    "ash_linear_backward_weight_scratch_bytes": (
+        _I64, [_I64, _I64, _I64, ctypes.c_int32, ctypes.c_int]
+    ),
+    "ash_linear_backward_weight": (
+        ctypes.c_int,
+        [ctypes.POINTER(_LinearArgs)] + [_PTR] * 5 + [_I64, ctypes.c_int] + [_PTR] * 3 + [_I64, _PTR],
+    ),
+    "ash_linear_second": (
+        ctypes.c_int,
+        [ctypes.POINTER(_LinearArgs), _PTR, _PTR, _I64, _PTR, _I64, _PTR, _PTR, _PTR],
+    ),
+    "ash_norm_forward": (ctypes.c_int, [ctypes.POINTER(_NormArgs), _PTR]),
+    "ash_norm_backward_scratch_bytes": (_I64, [_I64, _I64]),
+    "ash_norm_backward": (ctypes.c_int, [ctypes.POINTER(_NormArgs), _PTR]),
+    "ash_norm_second": (ctypes.c_int, [ctypes.POINTER(_NormArgs), _PTR]),
 }
 
 EXPORTED_SYMBOLS = tuple(_SIGNATURES)

@@ -20,11 +20,14 @@ OUT = os.path.join(OUT_DIR, "libash_hip.so")
 HOST_SOURCE = os.path.join(CSRC, "ash_host.cpp")
 HOST_OUT = os.path.join(OUT_DIR, "_ash_host.so")
 SOURCES = ["ash_map.hip", "ash_bulk.hip", "ash_query.hip", "ash_fusion.hip", "ash_mesh.hip",
-           "ash_rays.hip", "ash_conv.hip", "ash_surface.hip"]
+           "ash_rays.hip", "ash_conv.hip", "ash_surface.hip", "ash_layers.hip"]
 # compiled once for every width of rows (channels): device code of its own, which the
 # runtime loads where it is used
 ROWS_SOURCE, ROW_WIDTHS = "ash_rows.hip", (1, 2, 3, 4, 5, 6, 7, 8, 12, 16)
+# and once for every type of operands, by the header's ASH_* number
+LINEAR_SOURCE, LINEAR_DTYPES = "ash_linear.hip", (0, 2, 3, 4)
 HEADERS = [
+    os.path.join(CSRC, "ash_linear.h"),
     os.path.join(CSRC, "ash_probe.h"),
     os.path.join(CSRC, "ash_dev.h"),
     os.path.join(CSRC, "ash_query.h"),
@@ -61,7 +64,8 @@ def compile_flags():
 def units():
     """(source, object, flags of its own) of everything that is compiled."""
     return [(s, s.replace(".hip", ".o"), []) for s in SOURCES] + [
-        (ROWS_SOURCE, f"ash_rows_{width}.o", [f"-DASH_ROW_WIDTH={width}"]) for width in ROW_WIDTHS]
+        (ROWS_SOURCE, f"ash_rows_{width}.o", [f"-DASH_ROW_WIDTH={width}"]) for width in ROW_WIDTHS] + [
+        (LINEAR_SOURCE, f"ash_linear_{dtype}.o", [f"-DASH_LINEAR_DTYPE={dtype}"]) for dtype in LINEAR_DTYPES]
 
 
 def source_fingerprint() -> str:
@@ -101,7 +105,7 @@ def _older(out, deps) -> bool:
 
 
 def is_stale() -> bool:
-    return _older(OUT, [os.path.join(CSRC, s) for s in [*SOURCES, ROWS_SOURCE]] + HEADERS)
+    return _older(OUT, [os.path.join(CSRC, s) for s in [*SOURCES, ROWS_SOURCE, LINEAR_SOURCE]] + HEADERS)
 
 
 def host_is_stale() -> bool:

@@ -9,9 +9,11 @@
 // with their rows: 23 us of Python around 7 us of kernel).
 #include <torch/extension.h>
 
+#include <c10/hip/HIPGraphsC10Utils.h>
 #include <c10/hip/HIPStream.h>
 #include <torch/csrc/autograd/graph_task.h>
 #include <torch/csrc/autograd/python_function.h>
+#include <torch/csrc/autograd/variable.h>
 
 #include <dlfcn.h>
 
@@ -68,7 +70,16 @@ namespace py = pybind11;
     X(ash_query_forward)                                                              \
     X(ash_query_backward_forward)                                                     \
     X(ash_query_backward_forward_scaled)                                              \
-    X(ash_query_backward_backward_scaled)
+    X(ash_query_backward_backward_scaled)                                             \
+    X(ash_linear_forward)                                                             \
+    X(ash_linear_backward_input)                                                      \
+    X(ash_linear_backward_weight_scratch_bytes)                                       \
+    X(ash_linear_backward_weight)                                                     \
+    X(ash_linear_second)                                                              \
+    X(ash_norm_forward)                                                               \
+    X(ash_norm_backward_scratch_bytes)                                                \
+    X(ash_norm_backward)                                                              \
+    X(ash_norm_second)
 
 struct Library {
 #define X(name) decltype(&::name) name = nullptr;
@@ -961,6 +972,595 @@ Tensor query_gradient_later(const Tensor& gg_in, const Tensor& z_in, const std::
     return grad;
 }
 
+// -------------------------------------------------------- layers on features
+using torch::autograd::AutogradContext;
+using torch::autograd::variable_list;
+
+int32_t layer_dtype(const Tensor& t, const char* what) {
+    switch (t.scalar_type()) {
+        case at::kFloat: return ASH_F32;
+        case at::kBFloat16: return ASH_BF16;
+        case at::kHalf: return ASH_F16;
+        default:
+            fail(std::string(what) + " must be float32, bfloat16 or float16, got " + c10::toString(t.scalar_type()));
+    }
+}
+
+int32_t activation_of(const std::string& name) {
+    static const char* const kNames[] = {"none", "relu", "silu", "gelu", "softplus", "sine"};
+    for (int32_t i = ASH_ACT_NONE; i <= ASH_ACT_SINE; ++i) {
+        if (name == kNames[i]) return i;
+    }
+    fail("unknown activation '" + name + "': none, relu, silu, gelu, softplus or sine");
+}
+
+void on_device(const Tensor& t, const char* what, const Tensor& like) {
+    if (!t.is_cuda()) fail(std::string(what) + " must live on a HIP device, got " + t.device().str());
+    if (t.get_device() != like.get_device()) {
+        fail(std::string(what) + " is on " + t.device().str() + ", the input on " + like.device().str());
+    }
+}
+
+void of_type(const Tensor& t, const char* what, at::ScalarType type) {
+    if (t.scalar_type() != type) {
+        fail(std::string(what) + " must be " + c10::toString(type) + " like the output, got " +
+             c10::toString(t.scalar_type()));
+    }
+}
+
+// (rows, width) of a tensor whose last axis is a row.
+Tensor as_rows(const Tensor& t) { return t.dim() == 2 ? t : t.reshape({-1, t.size(-1)}); }
+
+// What the kernels read: values of a row consecutive, rows any number of values apart.
+Tensor readable(const Tensor& t) {
+    return t.dim() < 2 || (t.stride(-1) == 1 || t.size(-1) == 1) ? (t.dim() == 1 ? t.contiguous() : t)
+                                                                 : t.contiguous();
+}
+
+int64_t stride_of(const Tensor& t) { return t.defined() && t.dim() == 2 ? t.stride(0) : 0; }
+
+std::vector<int64_t> shape_with(const Tensor& input, int64_t width) {
+    std::vector<int64_t> shape = input.sizes().vec();
+    shape.back() = width;
+    return shape;
+}
+
+struct Activation {
+    int32_t kind;
+    double scale;
+    bool curved() const { return kind != ASH_ACT_NONE && kind != ASH_ACT_RELU; }
+};
+
+ash_linear_args linear_args(const Tensor& x, const Tensor& w, const Tensor& b, const Activation& f) {
+    ash_linear_args a{};
+    a.input = x.data_ptr();
+    a.weight = w.data_ptr();
+    a.bias = ptr<void>(b);
+    a.rows = x.size(0);
+    a.in_features = x.size(1);
+    a.out_features = w.size(0);
+    a.input_stride = x.stride(0);
+    a.dtype = a.out_dtype = layer_dtype(x, "input");
+    a.activation = f.kind;
+    a.activation_scale = static_cast<float>(f.scale);
+    return a;
+}
+
+Tensor linear_forward(const Tensor& x, const Tensor& w, const Tensor& b, const Tensor& residual,
+                      const Activation& f, Tensor* slope) {
+    const int64_t device = x.get_device();
+    ash_linear_args a = linear_args(x, w, b, f);
+    a.residual = ptr<void>(residual);
+    a.residual_stride = stride_of(residual);
+    Tensor out = empty({a.rows, a.out_features}, x.scalar_type(), device);
+    if (slope != nullptr) *slope = at::empty_like(out);
+    check(lib.ash_linear_forward(&a, out.data_ptr(), slope != nullptr ? slope->data_ptr() : nullptr,
+                                 stream_of(device)));
+    return out;
+}
+
+// (grad * slope) weight + addend
+Tensor linear_backward_input(const Tensor& grad, const Tensor& slope, const Tensor& w, const Tensor& addend) {
+    const int64_t device = grad.get_device();
+    ash_linear_args a{};
+    a.input = grad.data_ptr();   // not read
+    a.weight = w.data_ptr();
+    a.rows = grad.size(0);
+    a.in_features = w.size(1);
+    a.out_features = w.size(0);
+    a.dtype = a.out_dtype = layer_dtype(grad, "grad");
+    a.activation_scale = 1.0f;
+    Tensor out = empty({a.rows, a.in_features}, grad.scalar_type(), device);
+    check(lib.ash_linear_backward_input(&a, grad.data_ptr(), ptr<void>(slope), ptr<void>(addend), out.data_ptr(),
+                                        stream_of(device)));
+    return out;
+}
+
+// A factor of a weight's gradient: (grad * slope)^T input.
+struct Pair {
+    Tensor grad, slope, input;
+};
+
+// The sum of one or two pairs (the first defined); the bias' gradient is that of `biased`.
+std::pair<Tensor, Tensor> linear_backward_weight(const Pair& one, const Pair& two, bool second_has_bias,
+                                                 bool need_weight, bool need_bias) {
+    const Tensor& grad = one.grad;
+    const int64_t device = grad.get_device();
+    const bool pairs = two.grad.defined();
+    ash_linear_args a{};
+    a.input = a.weight = one.input.data_ptr();   // the weight is not read
+    a.rows = grad.size(0);
+    a.in_features = one.input.size(1);
+    a.out_features = grad.size(1);
+    a.input_stride = one.input.stride(0);
+    a.dtype = a.out_dtype = layer_dtype(grad, "grad");
+    a.activation_scale = 1.0f;
+    const Tensor gw = need_weight ? empty({a.out_features, a.in_features}, grad.scalar_type(), device) : Tensor();
+    const Tensor gb = need_bias ? empty({a.out_features}, grad.scalar_type(), device) : Tensor();
+    const int64_t bytes = lib.ash_linear_backward_weight_scratch_bytes(a.rows, a.in_features, a.out_features, a.dtype,
+                                                                       pairs ? 2 : 1);
+    const Tensor scratch = bytes > 0 ? empty({bytes}, at::kByte, device) : Tensor();
+    check(lib.ash_linear_backward_weight(&a, grad.data_ptr(), ptr<void>(one.slope), ptr<void>(two.grad),
+                                         ptr<void>(two.slope), ptr<void>(two.input), stride_of(two.input),
+                                         second_has_bias, ptr<void>(gw), ptr<void>(gb), ptr<void>(scratch), bytes,
+                                         stream_of(device)));
+    return {gw, gb};
+}
+
+// A backward pass that is captured into a graph while an eager graph of the same leaves
+// lives would hand their gradients to nodes of the default stream, which may not wait for
+// a stream that is being captured: the process ends there.  Refused here, where an error
+// can be caught.
+void leaves_may_be_captured(std::initializer_list<const Tensor*> tensors) {
+    if (c10::hip::currentStreamCaptureStatusMayInitCtx() == c10::hip::CaptureStatus::None) return;
+    for (const Tensor* t : tensors) {
+        if (!t->defined() || !t->requires_grad() || t->grad_fn()) continue;
+        const auto node = torch::autograd::impl::try_get_grad_accumulator(*t);
+        if (!node) continue;
+        const auto stream = node->stream();
+        need(!stream.has_value() || stream->id() != 0,
+             "a graph made before this capture still holds these leaves: delete what it computed first");
+    }
+}
+
+// The gradients of a dense layer as a node of their own, so that they have gradients too.
+// Tensors that are not there are not arguments of a node (torch numbers its edges by those
+// that are), hence the optionals, and it returns the gradients that are asked for only.
+struct LinearGrad : torch::autograd::Function<LinearGrad> {
+    static variable_list forward(AutogradContext* ctx, const Tensor& grad_in, const Tensor& x_in, const Tensor& w_in,
+                                 const Optional& b, const Optional& slope, int64_t kind, double scale, bool need_x,
+                                 bool need_w, bool need_b) {
+        const Tensor grad = grad_in.contiguous(), x = readable(x_in), w = w_in.contiguous();
+        const Tensor d = slope.value_or(Tensor());
+        ctx->save_for_backward({grad_in, x_in, w_in, b.value_or(Tensor()), d});
+        ctx->saved_data["kind"] = kind;
+        ctx->saved_data["scale"] = scale;
+        ctx->saved_data["needs"] = (need_x ? 1 : 0) | (need_w ? 2 : 0) | (need_b ? 4 : 0);
+        ctx->set_materialize_grads(false);
+        variable_list out;
+        if (need_x) out.push_back(linear_backward_input(grad, d, w, Tensor()));
+        if (need_w || need_b) {
+            auto [gw, gb] = linear_backward_weight({grad, d, x}, {}, false, need_w, need_b);
+            if (need_w) out.push_back(gw);
+            if (need_b) out.push_back(gb);
+        }
+        return out;
+    }
+
+    static variable_list backward(AutogradContext* ctx, variable_list grads) {
+        need(!at::GradMode::is_enabled(), "linear: gradients of third order are not computed");
+        const auto saved = ctx->get_saved_variables();
+        const Tensor grad = saved[0].contiguous(), x = readable(saved[1]), w = saved[2].contiguous();
+        const Tensor b = saved[3].defined() ? saved[3].contiguous() : Tensor(), d = saved[4];
+        const Activation f{static_cast<int32_t>(ctx->saved_data["kind"].toInt()), ctx->saved_data["scale"].toDouble()};
+        const int64_t needs = ctx->saved_data["needs"].toInt();
+        size_t next = 0;
+        const auto take = [&](int64_t bit) {
+            const Tensor t = needs & bit ? grads[next++] : Tensor();
+            return t.defined() ? t.contiguous() : t;
+        };
+        const Tensor u = take(1), of_w = take(2), of_b = take(4);
+        variable_list out(10);
+        if (!u.defined() && !of_w.defined() && !of_b.defined()) return out;
+        const bool need_grad = ctx->needs_input_grad(0), need_x = ctx->needs_input_grad(1),
+                   need_w = ctx->needs_input_grad(2), need_b = b.defined() && ctx->needs_input_grad(3);
+        const int64_t device = grad.get_device();
+        // t = u W^T + addend, addend = x V^T + c (in the operands' type: rounded once more)
+        Tensor addend;
+        if (of_w.defined()) addend = linear_forward(x, of_w, of_b, Tensor(), {ASH_ACT_NONE, 1.0}, nullptr);
+        else if (of_b.defined()) addend = of_b;
+        const bool bends = f.curved() && (need_x || need_w || need_b);
+        Tensor of_grad, q;
+        if (need_grad || bends) {
+            ash_linear_args a = linear_args(x, w, b, f);
+            if (need_grad) of_grad = empty({a.rows, a.out_features}, grad.scalar_type(), device);
+            if (bends) q = empty({a.rows, a.out_features}, grad.scalar_type(), device);
+            check(lib.ash_linear_second(&a, grad.data_ptr(), ptr<void>(u), stride_of(u), ptr<void>(addend),
+                                        stride_of(addend), ptr<void>(of_grad), ptr<void>(q), stream_of(device)));
+        }
+        out[0] = of_grad;
+        if (need_x) {
+            if (of_w.defined()) out[1] = linear_backward_input(grad, d, of_w, Tensor());
+            if (q.defined()) out[1] = linear_backward_input(q, Tensor(), w, out[1]);
+            if (!out[1].defined()) out[1] = at::zeros_like(x);
+        }
+        if (need_w || need_b) {
+            const Pair first{grad, d, u}, second{q, Tensor(), x};
+            std::pair<Tensor, Tensor> of{Tensor(), Tensor()};
+            const bool has_bias = need_b && q.defined();
+            if (u.defined() && need_w) of = linear_backward_weight(first, q.defined() ? second : Pair{}, has_bias, true, has_bias);
+            else if (q.defined()) of = linear_backward_weight(second, {}, false, need_w, has_bias);
+            if (need_w) out[2] = of.first.defined() ? of.first : at::zeros_like(w);
+            if (need_b) out[3] = of.second.defined() ? of.second : at::zeros_like(b);
+        }
+        return out;
+    }
+};
+
+struct Linear : torch::autograd::Function<Linear> {
+    static Tensor forward(AutogradContext* ctx, const Tensor& x_in, const Tensor& w_in, const Optional& b_in,
+                          const Optional& residual, int64_t kind, double scale) {
+        const Tensor x = readable(x_in), w = w_in.contiguous();
+        const Tensor b = b_in.has_value() ? b_in->contiguous() : Tensor();
+        const Activation f{static_cast<int32_t>(kind), scale};
+        const bool learns = x_in.requires_grad() || w_in.requires_grad() || (b_in.has_value() && b_in->requires_grad());
+        Tensor slope;
+        const Tensor out = linear_forward(x, w, b, residual.has_value() ? readable(*residual) : Tensor(), f,
+                                          learns && kind != ASH_ACT_NONE ? &slope : nullptr);
+        ctx->save_for_backward({x_in, w_in, b_in.value_or(Tensor()), slope});
+        ctx->saved_data["kind"] = kind;
+        ctx->saved_data["scale"] = scale;
+        ctx->saved_data["residual"] = residual.has_value();
+        ctx->set_materialize_grads(false);
+        return out;
+    }
+
+    static variable_list backward(AutogradContext* ctx, variable_list grads) {
+        variable_list out(6);
+        if (!grads[0].defined()) return out;
+        const auto saved = ctx->get_saved_variables();
+        const Tensor &x = saved[0], &w = saved[1], &b = saved[2], &slope = saved[3];
+        const bool need_x = ctx->needs_input_grad(0), need_w = ctx->needs_input_grad(1),
+                   need_b = b.defined() && ctx->needs_input_grad(2);
+        if (ctx->saved_data["residual"].toBool() && ctx->needs_input_grad(b.defined() ? 3 : 2)) out[3] = grads[0];
+        if (!need_x && !need_w && !need_b) return out;
+        if (at::GradMode::is_enabled()) {
+            const auto got = LinearGrad::apply(grads[0], x, w, maybe(b), maybe(slope), ctx->saved_data["kind"].toInt(),
+                                               ctx->saved_data["scale"].toDouble(), need_x, need_w, need_b);
+            size_t next = 0;
+            if (need_x) out[0] = got[next++];
+            if (need_w) out[1] = got[next++];
+            if (need_b) out[2] = got[next++];
+            return out;
+        }
+        const Tensor grad = grads[0].contiguous();
+        if (need_x) out[0] = linear_backward_input(grad, slope, w.contiguous(), Tensor());
+        if (need_w || need_b) {
+            std::tie(out[1], out[2]) = linear_backward_weight({grad, slope, readable(x)}, {}, false, need_w, need_b);
+        }
+        return out;
+    }
+};
+
+void check_features(const Tensor& x, const Tensor& w) {
+    if (x.dim() < 1 || w.dim() != 2 || x.size(-1) != w.size(1)) {
+        fail("linear: weight must be (out, " + (x.dim() < 1 ? std::string("in") : std::to_string(x.size(-1))) +
+             ") for rows of an input " + shape_of(x) + ", got " + shape_of(w));
+    }
+    need(w.size(0) >= 1 && w.size(1) >= 1, "linear: at least one feature in and one out");
+}
+
+void check_epilogue(const Optional& b, const Optional& residual, const Tensor& x, const Tensor& w, at::ScalarType type) {
+    if (b.has_value()) {
+        if (b->dim() != 1 || b->size(0) != w.size(0)) {
+            fail("linear: bias must be (" + std::to_string(w.size(0)) + ",), got " + shape_of(*b));
+        }
+        of_type(*b, "linear: bias", type);
+        on_device(*b, "linear: bias", x);
+    }
+    if (residual.has_value()) {
+        of_type(*residual, "linear: residual", type);
+        on_device(*residual, "linear: residual", x);
+    }
+}
+
+Optional rows_of_residual(const Optional& residual, const std::vector<int64_t>& shape) {
+    if (!residual.has_value()) return residual;
+    Tensor r = *residual;
+    if (r.sizes() != at::IntArrayRef(shape)) {
+        bool fits = r.dim() <= static_cast<int64_t>(shape.size());
+        for (int64_t d = 1; fits && d <= r.dim(); ++d) fits = r.size(-d) == 1 || r.size(-d) == shape[shape.size() - d];
+        if (!fits) {
+            std::string out = "(";
+            for (const int64_t n : shape) out += std::to_string(n) + ", ";
+            fail("residual " + shape_of(r) + " does not broadcast to the output " + out.substr(0, out.size() - 2) + ")");
+        }
+        r = r.expand(shape);
+    }
+    return r.dim() == 2 ? r : r.reshape({-1, shape.back()});
+}
+
+Tensor linear(const Tensor& x, const Tensor& w, const Optional& b, const std::string& activation, double scale,
+              const Optional& residual) {
+    check_features(x, w);
+    const Activation f{activation_of(activation), scale};
+    layer_dtype(x, "linear: input");
+    of_type(w, "linear: weight", x.scalar_type());
+    on_device(x, "linear: input", x);
+    on_device(w, "linear: weight", x);
+    check_epilogue(b, residual, x, w, x.scalar_type());
+    const auto shape = shape_with(x, w.size(0));
+    const Tensor rows = as_rows(x);
+    const Optional r = rows_of_residual(residual, shape);
+    const bool learns = at::GradMode::is_enabled() &&
+                        (x.requires_grad() || w.requires_grad() || (b.has_value() && b->requires_grad()) ||
+                         (r.has_value() && r->requires_grad()));
+    if (learns) leaves_may_be_captured({&x, &w, b.has_value() ? &*b : &x, residual.has_value() ? &*residual : &x});
+    const Tensor out = learns ? Linear::apply(rows, w, b, r, f.kind, f.scale)
+                              : linear_forward(readable(rows), w.contiguous(), b.has_value() ? b->contiguous() : Tensor(),
+                                               r.has_value() ? readable(*r) : Tensor(), f, nullptr);
+    return x.dim() == 2 ? out : out.reshape(shape);
+}
+
+constexpr auto kE4m3 = at::ScalarType::Float8_e4m3fn;
+
+// 8-bit rows (values, scales), as QuantizedRows holds them.
+void check_quantized(const Tensor& values, const Tensor& scales, const char* what) {
+    if (values.scalar_type() != kE4m3 || values.dim() < 1) fail(std::string(what) + " must be rows of float8_e4m3fn");
+    if (scales.scalar_type() != at::kFloat || scales.sizes() != values.sizes().slice(0, values.dim() - 1)) {
+        fail(std::string(what) + " needs one float32 scale a row, got " + c10::toString(scales.scalar_type()) + " " +
+             shape_of(scales) + " for " + shape_of(values));
+    }
+}
+
+Tensor linear_quantized(const Tensor& x, const Tensor& x_scales, const Tensor& w, const Tensor& w_scales,
+                        const Optional& b, const std::string& activation, double scale, const Optional& residual,
+                        const std::optional<at::ScalarType>& out_dtype) {
+    check_quantized(x, x_scales, "linear: input");
+    check_quantized(w, w_scales, "linear: weight");
+    check_features(x, w);
+    const Activation f{activation_of(activation), scale};
+    const at::ScalarType type = out_dtype.has_value() ? *out_dtype
+                                : b.has_value()       ? b->scalar_type()
+                                : residual.has_value() ? residual->scalar_type()
+                                                       : at::kBFloat16;
+    need(type == at::kFloat || type == at::kBFloat16 || type == at::kHalf,
+         "linear: the output of 8-bit rows is float32, bfloat16 or float16");
+    on_device(x, "linear: input", x);
+    on_device(x_scales, "linear: the input's scales", x);
+    on_device(w, "linear: weight", x);
+    on_device(w_scales, "linear: the weight's scales", x);
+    check_epilogue(b, residual, x, w, type);
+    need(!at::GradMode::is_enabled() || !((b.has_value() && b->requires_grad()) ||
+                                          (residual.has_value() && residual->requires_grad()) ||
+                                          x_scales.requires_grad() || w_scales.requires_grad()),
+         "linear: 8-bit rows have no gradients; call it under torch.no_grad()");
+    const auto shape = shape_with(x, w.size(0));
+    const int64_t device = x.get_device();
+    const Tensor rows = readable(as_rows(x)), weight = w.contiguous(), bias = b.has_value() ? b->contiguous() : Tensor();
+    const Tensor rows_scales = x_scales.contiguous(), weight_scales = w_scales.contiguous();
+    const Optional r = rows_of_residual(residual, shape);
+    const Tensor more = r.has_value() ? readable(*r) : Tensor();
+    ash_linear_args a{};
+    a.input = rows.data_ptr();
+    a.weight = weight.data_ptr();
+    a.bias = ptr<void>(bias);
+    a.residual = ptr<void>(more);
+    a.input_scales = ptr<float>(rows_scales);
+    a.weight_scales = ptr<float>(weight_scales);
+    a.rows = rows.size(0);
+    a.in_features = w.size(1);
+    a.out_features = w.size(0);
+    a.input_stride = rows.stride(0);
+    a.residual_stride = stride_of(more);
+    a.dtype = ASH_E4M3;
+    a.out_dtype = type == at::kFloat ? ASH_F32 : type == at::kHalf ? ASH_F16 : ASH_BF16;
+    a.activation = f.kind;
+    a.activation_scale = static_cast<float>(f.scale);
+    Tensor out = empty(shape, type, device);
+    check(lib.ash_linear_forward(&a, out.data_ptr(), nullptr, stream_of(device)));
+    return out;
+}
+
+// ------------------------------------------------------------------------ norm
+constexpr int64_t kMaxNormColumns = 16384;   // ash_norm_args
+
+ash_norm_args norm_args(const Tensor& x, const Tensor& w, double eps) {
+    ash_norm_args a{};
+    a.input = x.data_ptr();
+    a.weight = ptr<void>(w);
+    a.rows = x.size(0);
+    a.cols = x.size(1);
+    a.input_stride = x.stride(0);
+    a.dtype = layer_dtype(x, "input");
+    a.normalise = 1;
+    a.eps = static_cast<float>(eps);
+    return a;
+}
+
+struct Normed {
+    Tensor y, sum, scales;
+};
+
+Normed norm_forward(const Tensor& x, const Tensor& w, const Tensor& residual, double eps, bool normalise, bool quantize) {
+    const int64_t device = x.get_device();
+    ash_norm_args a = norm_args(x, w, eps);
+    a.normalise = normalise;
+    Normed out;
+    out.y = empty({a.rows, a.cols}, quantize ? kE4m3 : x.scalar_type(), device);
+    a.output = out.y.data_ptr();
+    if (residual.defined()) {
+        a.residual = residual.data_ptr();
+        a.residual_stride = residual.stride(0);
+        out.sum = empty({a.rows, a.cols}, x.scalar_type(), device);
+        a.sum_out = out.sum.data_ptr();
+    }
+    if (quantize) {
+        out.scales = empty({a.rows}, at::kFloat, device);
+        a.scales = ptr<float>(out.scales);
+    }
+    check(lib.ash_norm_forward(&a, stream_of(device)));
+    return out;
+}
+
+Tensor norm_scratch(const ash_norm_args& a, int64_t device) {
+    const int64_t bytes = lib.ash_norm_backward_scratch_bytes(a.rows, a.cols);
+    return empty({std::max<int64_t>(bytes / 4, 1)}, at::kFloat, device);
+}
+
+std::pair<Tensor, Tensor> norm_backward(const Tensor& grad, const Tensor& grad_sum, const Tensor& s, const Tensor& w,
+                                        double eps, bool need_s, bool need_w) {
+    const int64_t device = s.get_device();
+    ash_norm_args a = norm_args(s, w, eps);
+    a.grad = grad.data_ptr();
+    a.grad_sum = ptr<void>(grad_sum);
+    const Tensor gs = need_s ? empty({a.rows, a.cols}, s.scalar_type(), device) : Tensor();
+    const Tensor gw = need_w ? empty({a.cols}, s.scalar_type(), device) : Tensor();
+    const Tensor scratch = need_w ? norm_scratch(a, device) : Tensor();
+    a.output = ptr<void>(gs);
+    a.weight_out = ptr<void>(gw);
+    a.parts = ptr<float>(scratch);
+    check(lib.ash_norm_backward(&a, stream_of(device)));
+    return {gs, gw};
+}
+
+// As LinearGrad: the gradients of the norm, with gradients of their own.
+struct NormGrad : torch::autograd::Function<NormGrad> {
+    static variable_list forward(AutogradContext* ctx, const Tensor& grad, const Tensor& s, const Optional& w_in,
+                                 double eps, bool need_s, bool need_w) {
+        const Tensor w = w_in.value_or(Tensor());
+        ctx->save_for_backward({grad, s, w});
+        ctx->saved_data["eps"] = eps;
+        ctx->saved_data["needs"] = (need_s ? 1 : 0) | (need_w ? 2 : 0);
+        ctx->set_materialize_grads(false);
+        auto [gs, gw] = norm_backward(grad.contiguous(), Tensor(), readable(s), w.defined() ? w.contiguous() : w, eps,
+                                      need_s, need_w);
+        variable_list out;
+        if (need_s) out.push_back(gs);
+        if (need_w) out.push_back(gw);
+        return out;
+    }
+
+    static variable_list backward(AutogradContext* ctx, variable_list grads) {
+        need(!at::GradMode::is_enabled(), "rms_norm: gradients of third order are not computed");
+        const auto saved = ctx->get_saved_variables();
+        const int64_t needs = ctx->saved_data["needs"].toInt();
+        const Tensor of_s = needs & 1 ? grads[0] : Tensor(), of_w = needs & 2 ? grads.back() : Tensor();
+        variable_list out(6);
+        if (!of_s.defined() && !of_w.defined()) return out;
+        const Tensor grad = saved[0].contiguous(), s = readable(saved[1]);
+        const Tensor w = saved[2].defined() ? saved[2].contiguous() : Tensor();
+        const Tensor u = of_s.defined() ? of_s.contiguous() : of_s, v = of_w.defined() ? of_w.contiguous() : of_w;
+        const bool need_w = w.defined() && ctx->needs_input_grad(2);
+        const int64_t device = s.get_device();
+        ash_norm_args a = norm_args(s, w, ctx->saved_data["eps"].toDouble());
+        a.grad = grad.data_ptr();
+        a.second = ptr<void>(u);
+        a.second_weight = ptr<void>(v);
+        if (ctx->needs_input_grad(0)) out[0] = empty({a.rows, a.cols}, s.scalar_type(), device);
+        if (ctx->needs_input_grad(1)) out[1] = empty({a.rows, a.cols}, s.scalar_type(), device);
+        if (need_w) out[2] = empty({a.cols}, s.scalar_type(), device);
+        const Tensor scratch = need_w ? norm_scratch(a, device) : Tensor();
+        a.grad_out = ptr<void>(out[0]);
+        a.output = ptr<void>(out[1]);
+        a.weight_out = ptr<void>(out[2]);
+        a.parts = ptr<float>(scratch);
+        check(lib.ash_norm_second(&a, stream_of(device)));
+        return out;
+    }
+};
+
+struct Norm : torch::autograd::Function<Norm> {
+    // y, and the sum where there is a residual
+    static variable_list forward(AutogradContext* ctx, const Tensor& x_in, const Optional& w_in, const Optional& residual,
+                                 double eps) {
+        const Tensor x = readable(x_in), w = w_in.has_value() ? w_in->contiguous() : Tensor();
+        const Normed out = norm_forward(x, w, residual.has_value() ? readable(*residual) : Tensor(), eps, true, false);
+        ctx->save_for_backward({out.sum.defined() ? out.sum : x_in, w_in.value_or(Tensor())});
+        ctx->saved_data["eps"] = eps;
+        ctx->saved_data["residual"] = residual.has_value();
+        ctx->set_materialize_grads(false);
+        if (out.sum.defined()) return {out.y, out.sum};
+        return {out.y};
+    }
+
+    static variable_list backward(AutogradContext* ctx, variable_list grads) {
+        variable_list out(4);
+        const auto saved = ctx->get_saved_variables();
+        const Tensor &s = saved[0], &w = saved[1];
+        const bool residual = ctx->saved_data["residual"].toBool();
+        const bool need_x = ctx->needs_input_grad(0), need_w = w.defined() && ctx->needs_input_grad(1);
+        const bool need_r = residual && ctx->needs_input_grad(w.defined() ? 2 : 1);
+        const Tensor grad = grads[0], grad_sum = residual ? grads[1] : Tensor();
+        Tensor gs, gw;
+        if (!grad.defined()) {
+            gs = grad_sum;   // only the sum was used
+        } else if (at::GradMode::is_enabled()) {
+            if (need_x || need_r || need_w) {
+                const auto got = NormGrad::apply(grad, s, maybe(w), ctx->saved_data["eps"].toDouble(), need_x || need_r, need_w);
+                if (need_x || need_r) gs = grad_sum.defined() ? got[0] + grad_sum : got[0];
+                if (need_w) gw = got.back();
+            }
+        } else if (need_x || need_r || need_w) {
+            std::tie(gs, gw) = norm_backward(grad.contiguous(), grad_sum.defined() ? grad_sum.contiguous() : grad_sum,
+                                             readable(s), w.defined() ? w.contiguous() : w,
+                                             ctx->saved_data["eps"].toDouble(), need_x || need_r, need_w);
+        }
+        if (need_x) out[0] = gs;
+        if (need_w) out[1] = gw;
+        if (need_r) out[2] = gs;
+        return out;
+    }
+};
+
+// (y, sum or None, scales or None)
+std::tuple<Tensor, Optional, Optional> rms_norm(const Tensor& x, const Optional& w, const Optional& residual, double eps,
+                                                bool quantize) {
+    layer_dtype(x, "rms_norm: input");
+    if (x.dim() < 1 || x.size(-1) < 1 || x.size(-1) > kMaxNormColumns) {
+        fail("rms_norm takes rows of 1 to 16384 values, got " + shape_of(x));
+    }
+    need(eps >= 0.0, "rms_norm: eps must not be negative");
+    on_device(x, "rms_norm: input", x);
+    if (w.has_value()) {
+        if (w->dim() != 1 || w->size(0) != x.size(-1)) {
+            fail("rms_norm: weight must be (" + std::to_string(x.size(-1)) + ",), got " + shape_of(*w));
+        }
+        of_type(*w, "rms_norm: weight", x.scalar_type());
+        on_device(*w, "rms_norm: weight", x);
+    }
+    if (residual.has_value()) {
+        of_type(*residual, "rms_norm: residual", x.scalar_type());
+        on_device(*residual, "rms_norm: residual", x);
+    }
+    const auto shape = x.sizes().vec();
+    const Tensor rows = as_rows(x);
+    const Optional r = rows_of_residual(residual, shape);
+    const bool learns = at::GradMode::is_enabled() && (x.requires_grad() || (w.has_value() && w->requires_grad()) ||
+                                                       (r.has_value() && r->requires_grad()));
+    const auto back = [&](const Tensor& t) { return x.dim() == 2 ? t : t.reshape(shape); };
+    if (learns) {
+        need(!quantize, "rms_norm: 8-bit rows have no gradients; call it under torch.no_grad()");
+        leaves_may_be_captured({&x, w.has_value() ? &*w : &x, residual.has_value() ? &*residual : &x});
+        const variable_list out = Norm::apply(rows, w, r, eps);
+        return {back(out[0]), out.size() > 1 ? Optional(back(out[1])) : std::nullopt, std::nullopt};
+    }
+    const Normed out = norm_forward(readable(rows), w.has_value() ? w->contiguous() : Tensor(),
+                                    r.has_value() ? readable(*r) : Tensor(), eps, true, quantize);
+    return {back(out.y), out.sum.defined() ? Optional(back(out.sum)) : std::nullopt,
+            quantize ? Optional(out.scales.reshape(x.sizes().slice(0, x.dim() - 1))) : std::nullopt};
+}
+
+std::pair<Tensor, Tensor> quantize_rows(const Tensor& x) {
+    layer_dtype(x, "QuantizedRows: rows");
+    if (x.dim() < 1 || x.size(-1) < 1 || x.size(-1) > kMaxNormColumns) {
+        fail("QuantizedRows takes rows of 1 to 16384 values, got " + shape_of(x));
+    }
+    on_device(x, "QuantizedRows: rows", x);
+    const Normed out = norm_forward(readable(as_rows(x)), Tensor(), Tensor(), 0.0, false, true);
+    return {out.y.reshape(x.sizes()), out.scales.reshape(x.sizes().slice(0, x.dim() - 1))};
+}
+
 // Whether nobody looks at the gradient that the node of `ctx` hands to the node
 // behind its input `input`: no hook behind the one or before the other.
 bool hands_over_unseen(const py::object& ctx, size_t input) {
@@ -1046,6 +1646,10 @@ PYBIND11_MODULE(_ash_host, m) {
     m.def("query_gradient_later", &query_gradient_later);
     m.def("hands_over_unseen", &hands_over_unseen);
     m.def("grad_requested", &grad_requested);
+    m.def("linear", &linear);
+    m.def("linear_quantized", &linear_quantized);
+    m.def("rms_norm", &rms_norm);
+    m.def("quantize_rows", &quantize_rows);
     m.def("query_backward_backward", &query_backward_backward, arg("grad_grad_offsets"), arg("z"),
           arg("operands"), arg("interpolation"), arg("need_z"), arg("need_embeddings"),
           arg("accumulate_into"), arg("cell_size") = 1.0);

@@ -1,0 +1,57 @@
+// What the kernels of a dense layer (ash_linear.hip, compiled once for every type of
+// operands) and its C ABI (ash_layers.hip) share.
+#pragma once
+
+#include "ash_table.h"
+
+#include "../../include/ash_hip.h"
+
+namespace ash {
+
+// One product  out[r, c] = sum_k P[r, k] Q[c, k]  and what becomes of it.
+//   forward      P = input (rows x in),   Q = weight (out x in)
+//   grad input   P = gz (rows x out),     Q = weight transposed (in x out)
+//   grad weight  P = gz transposed (out x rows), Q = input transposed (in x rows)
+// with gz = grad * slope, formed as the operand is read.
+struct LinearJob {
+    const void* input;
+    const void* weight;
+    const void* bias;
+    const void* residual;
+    const void* grad;         // gradients only: of the output
+    const void* slope;        // f'(z) as the forward left it, or null: one
+    const float* input_scales;
+    const float* weight_scales;
+    void* out;
+    void* slope_out;
+    int64_t rows, in, cols;   // cols: out features
+    int64_t input_stride, residual_stride;
+    int32_t out_dtype, activation;
+    float act_scale;
+    // second order: the gradient of the gradient of the input, an addend, and where t grad
+    // f''(z) goes; `out` takes the gradient of `grad`
+    const void* second_input;
+    const void* addend;
+    int64_t addend_stride;
+    void* curvature_out;
+    // weight's gradient: a second pair of operands whose product is added
+    const void* second_grad;
+    const void* second_slope;
+    const void* second_factor;
+    int64_t second_stride;
+    bool second_has_bias;     // which pair's grad the bias' gradient sums
+    void* bias_out;
+    void* scratch;
+    int32_t splits;           // parts the rows are cut into, per pair
+};
+
+enum LinearKind { kLinearForward, kLinearGradInput, kLinearGradWeight, kLinearSecond };
+
+// Defined in ash_linear.hip, one set for every type.
+template <int DTYPE>
+int linear_run(LinearKind kind, const LinearJob& job, hipStream_t s);
+
+// Parts that the rows are cut into for a weight's gradient (ash_layers.hip).
+int32_t linear_splits(int64_t rows, int64_t in, int64_t out, int32_t dtype, int pairs);
+
+}  // namespace ash
