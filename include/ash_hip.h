@@ -967,17 +967,25 @@ typedef struct ash_linear_args {
     float activation_scale;
 } ash_linear_args;
 
-/* slope: f'(z), for the backward calls, or NULL. */
+/* slope: f'(z) for the backward calls, or NULL; float32, for ASH_BF16 float16, and
+ * of SINE without its factor a. */
 int ash_linear_forward(const ash_linear_args* args, void* output, void* slope, void* stream);
 /* grad_input = (grad * slope) weight (+ addend); slope NULL: f'(z) is one.  Reads
- * weight and the sizes of args. */
+ * weight, the activation (whose factor a slope is without) and the sizes of args. */
 int ash_linear_backward_input(const ash_linear_args* args, const void* grad, const void* slope,
                               const void* addend, void* grad_input, void* stream);
+/* scaled = grad * slope (and the activation's factor), rounded to dtype: what the
+ * backward calls form of their operands as they read them, for sizes at which it pays
+ * to form it once for both (`wants`: 1) and pass it with slope NULL. */
+int ash_linear_wants_scaled_gradient(int64_t rows, int64_t in_features, int64_t out_features,
+                                     int32_t dtype);
+int ash_linear_scale_gradient(const ash_linear_args* args, const void* grad, const void* slope,
+                              void* scaled, void* stream);
 /* grad_weight = (grad * slope)^T input and grad_bias = the column sums of grad *
  * slope, either NULL.  With second_grad, (second_grad * second_slope)^T second_input
  * is added, and second_has_bias says which of the two the bias' gradient sums.  The
  * rows are cut into parts whose sums meet in scratch and are joined in their order:
- * the same numbers on every run.  Reads input and the sizes of args. */
+ * the same numbers on every run.  Reads input, the activation and the sizes of args. */
 int64_t ash_linear_backward_weight_scratch_bytes(int64_t rows, int64_t in_features,
                                                  int64_t out_features, int32_t dtype, int pairs);
 int ash_linear_backward_weight(const ash_linear_args* args, const void* grad, const void* slope,

@@ -13,6 +13,7 @@ import torch
 
 F32 = 2.0**-24
 SLACK = 16
+SLOPE = {torch.bfloat16: torch.float16}
 
 
 def half(dtype):
@@ -115,8 +116,9 @@ def linear(x, w, b, kind="none", a=1.0, residual=None, x_scales=None, w_scales=N
 
 
 def linear_gradients(gy, x, w, d, kind, dtype):
-    """(gx, gw, gb): the slope is kept, and its product with gy formed, in the type."""
-    gz = Off(gy) if kind == "none" else (Off(gy) * d.rounded(dtype)).rounded(dtype)
+    """(gx, gw, gb, gz): the slope is kept in float32 (fp16 for bf16, of a sine without its
+    factor) and its product with gy rounded to the type."""
+    gz = Off(gy) if kind == "none" else (Off(gy) * d.rounded(SLOPE.get(dtype, torch.float32))).rounded(dtype)
     return gz @ Off(w), gz.t() @ Off(x), gz.column_sums(), gz
 
 

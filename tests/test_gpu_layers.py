@@ -49,6 +49,26 @@ def test_linear_and_its_gradients(gpu_ash, shape, dtype):
         ref.check(have, want, dtype, what)
 
 
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16], ids=ids)
+@pytest.mark.parametrize("rows,k,m,kind", [(16640, 1032, 1000, "gelu"), (20001, 520, 776, "none"),
+                                           (33000, 256, 512, "sine"), (4100, 2056, 544, "silu")])
+def test_linear_and_its_gradients_in_large_tiles(gpu_ash, rows, k, m, kind, dtype):
+    """Sizes that end inside a tile and inside a step, an odd number of steps; aligned
+    and not (the other tiles take those)."""
+    a = 30.0 if kind == "sine" else 1.0
+    x, w, b, r, gy, _ = operands(rows, k + 1, m, dtype, seed=20, a=a, sine=kind == "sine")
+    w, wide = w[:, :k].contiguous(), torch.cat([x, x[:, :7]], 1)
+    for x in (x[:, :k].contiguous(), wide[:, :k], x[:, 1:]):
+        y, d, _, _ = ref.linear(x, w, b, kind, a, r)
+        gx, gw, gb, _ = ref.linear_gradients(gy, x, w, d, kind, dtype)
+        lx, lw, lb = leaves(x, w, b)
+        out = gpu_ash.linear(lx, lw, lb, activation=kind, scale=a, residual=r)
+        ref.check(out, y, dtype, "forward")
+        got = torch.autograd.grad(out, [lx, lw, lb], gy)
+        for have, want, what in zip(got, (gx, gw, gb), ("gx", "gw", "gb")):
+            ref.check(have, want, dtype, what)
+
+
 @pytest.mark.parametrize("dtype", TYPES, ids=ids)
 @pytest.mark.parametrize("kind,a", ACTS)
 def test_activations(gpu_ash, kind, a, dtype):
@@ -257,7 +277,7 @@ def test_rows_beyond_32_bits(gpu_ash):
 # --------------------------------------------------------------------- 8-bit rows
 @pytest.mark.parametrize("out_dtype", TYPES, ids=ids)
 @pytest.mark.parametrize("shape", [(1, 16, 1), (1, 1024, 64), (7, 3, 5), (16, 131, 33), (40, 600, 48), (65, 128, 64),
-                                   (130, 67, 129), (1000, 257, 300)], ids=str)
+                                   (130, 67, 129), (1000, 257, 300), (16500, 400, 1008)], ids=str)
 def test_linear_of_8_bit_rows(gpu_ash, shape, out_dtype):
     rows, k, m = shape
     x, w, b, r, _, _ = operands(rows, k, m, torch.float32, seed=11)

@@ -74,7 +74,7 @@ def linear(
 
     Gradients of first and second order exist for every operand (of the gradient
     of a weight too, not of third order).  For them the forward keeps the slope of
-    the activation at every output, in the operands' type.  They are the same
+    the activation at every output, in float32 (float16 for bfloat16 operands).  They are the same
     numbers on every run.
 
     With 8-bit rows (`QuantizedRows`, both or neither) every sum of products is

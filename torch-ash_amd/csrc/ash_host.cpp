@@ -73,6 +73,8 @@ namespace py = pybind11;
     X(ash_query_backward_backward_scaled)                                             \
     X(ash_linear_forward)                                                             \
     X(ash_linear_backward_input)                                                      \
+    X(ash_linear_wants_scaled_gradient)                                               \
+    X(ash_linear_scale_gradient)                                                      \
     X(ash_linear_backward_weight_scratch_bytes)                                       \
     X(ash_linear_backward_weight)                                                     \
     X(ash_linear_second)                                                              \
@@ -1053,14 +1055,32 @@ Tensor linear_forward(const Tensor& x, const Tensor& w, const Tensor& b, const T
     a.residual = ptr<void>(residual);
     a.residual_stride = stride_of(residual);
     Tensor out = empty({a.rows, a.out_features}, x.scalar_type(), device);
-    if (slope != nullptr) *slope = at::empty_like(out);
+    if (slope != nullptr) {
+        *slope = empty({a.rows, a.out_features}, x.scalar_type() == at::kBFloat16 ? at::kHalf : at::kFloat, device);
+    }
     check(lib.ash_linear_forward(&a, out.data_ptr(), slope != nullptr ? slope->data_ptr() : nullptr,
                                  stream_of(device)));
     return out;
 }
 
+// Where both backward calls are better off with grad * slope formed once: that, and no
+// slope any more.
+void scale_gradient(Tensor& grad, Tensor& slope, const Tensor& x, const Tensor& w, const Activation& f) {
+    if (!slope.defined() || !lib.ash_linear_wants_scaled_gradient(grad.size(0), w.size(1), w.size(0),
+                                                                  layer_dtype(grad, "grad"))) {
+        return;
+    }
+    ash_linear_args a = linear_args(x, w, Tensor(), f);
+    const Tensor scaled = at::empty_like(grad);
+    check(lib.ash_linear_scale_gradient(&a, grad.data_ptr(), slope.data_ptr(), scaled.data_ptr(),
+                                        stream_of(grad.get_device())));
+    grad = scaled;
+    slope = Tensor();
+}
+
 // (grad * slope) weight + addend
-Tensor linear_backward_input(const Tensor& grad, const Tensor& slope, const Tensor& w, const Tensor& addend) {
+Tensor linear_backward_input(const Tensor& grad, const Tensor& slope, const Tensor& w, const Tensor& addend,
+                             const Activation& f) {
     const int64_t device = grad.get_device();
     ash_linear_args a{};
     a.input = grad.data_ptr();   // not read
@@ -1069,7 +1089,8 @@ Tensor linear_backward_input(const Tensor& grad, const Tensor& slope, const Tens
     a.in_features = w.size(1);
     a.out_features = w.size(0);
     a.dtype = a.out_dtype = layer_dtype(grad, "grad");
-    a.activation_scale = 1.0f;
+    a.activation = f.kind;
+    a.activation_scale = static_cast<float>(f.scale);
     Tensor out = empty({a.rows, a.in_features}, grad.scalar_type(), device);
     check(lib.ash_linear_backward_input(&a, grad.data_ptr(), ptr<void>(slope), ptr<void>(addend), out.data_ptr(),
                                         stream_of(device)));
@@ -1083,7 +1104,7 @@ struct Pair {
 
 // The sum of one or two pairs (the first defined); the bias' gradient is that of `biased`.
 std::pair<Tensor, Tensor> linear_backward_weight(const Pair& one, const Pair& two, bool second_has_bias,
-                                                 bool need_weight, bool need_bias) {
+                                                 bool need_weight, bool need_bias, const Activation& f) {
     const Tensor& grad = one.grad;
     const int64_t device = grad.get_device();
     const bool pairs = two.grad.defined();
@@ -1094,7 +1115,8 @@ std::pair<Tensor, Tensor> linear_backward_weight(const Pair& one, const Pair& tw
     a.out_features = grad.size(1);
     a.input_stride = one.input.stride(0);
     a.dtype = a.out_dtype = layer_dtype(grad, "grad");
-    a.activation_scale = 1.0f;
+    a.activation = f.kind;
+    a.activation_scale = static_cast<float>(f.scale);
     const Tensor gw = need_weight ? empty({a.out_features, a.in_features}, grad.scalar_type(), device) : Tensor();
     const Tensor gb = need_bias ? empty({a.out_features}, grad.scalar_type(), device) : Tensor();
     const int64_t bytes = lib.ash_linear_backward_weight_scratch_bytes(a.rows, a.in_features, a.out_features, a.dtype,
@@ -1132,15 +1154,16 @@ struct LinearGrad : torch::autograd::Function<LinearGrad> {
                                  bool need_w, bool need_b) {
         const Tensor grad = grad_in.contiguous(), x = readable(x_in), w = w_in.contiguous();
         const Tensor d = slope.value_or(Tensor());
+        const Activation f{static_cast<int32_t>(kind), scale};
         ctx->save_for_backward({grad_in, x_in, w_in, b.value_or(Tensor()), d});
         ctx->saved_data["kind"] = kind;
         ctx->saved_data["scale"] = scale;
         ctx->saved_data["needs"] = (need_x ? 1 : 0) | (need_w ? 2 : 0) | (need_b ? 4 : 0);
         ctx->set_materialize_grads(false);
         variable_list out;
-        if (need_x) out.push_back(linear_backward_input(grad, d, w, Tensor()));
+        if (need_x) out.push_back(linear_backward_input(grad, d, w, Tensor(), f));
         if (need_w || need_b) {
-            auto [gw, gb] = linear_backward_weight({grad, d, x}, {}, false, need_w, need_b);
+            auto [gw, gb] = linear_backward_weight({grad, d, x}, {}, false, need_w, need_b, f);
             if (need_w) out.push_back(gw);
             if (need_b) out.push_back(gb);
         }
@@ -1180,16 +1203,16 @@ struct LinearGrad : torch::autograd::Function<LinearGrad> {
         }
         out[0] = of_grad;
         if (need_x) {
-            if (of_w.defined()) out[1] = linear_backward_input(grad, d, of_w, Tensor());
-            if (q.defined()) out[1] = linear_backward_input(q, Tensor(), w, out[1]);
+            if (of_w.defined()) out[1] = linear_backward_input(grad, d, of_w, Tensor(), f);
+            if (q.defined()) out[1] = linear_backward_input(q, Tensor(), w, out[1], f);
             if (!out[1].defined()) out[1] = at::zeros_like(x);
         }
         if (need_w || need_b) {
             const Pair first{grad, d, u}, second{q, Tensor(), x};
             std::pair<Tensor, Tensor> of{Tensor(), Tensor()};
             const bool has_bias = need_b && q.defined();
-            if (u.defined() && need_w) of = linear_backward_weight(first, q.defined() ? second : Pair{}, has_bias, true, has_bias);
-            else if (q.defined()) of = linear_backward_weight(second, {}, false, need_w, has_bias);
+            if (u.defined() && need_w) of = linear_backward_weight(first, q.defined() ? second : Pair{}, has_bias, true, has_bias, f);
+            else if (q.defined()) of = linear_backward_weight(second, {}, false, need_w, has_bias, f);
             if (need_w) out[2] = of.first.defined() ? of.first : at::zeros_like(w);
             if (need_b) out[3] = of.second.defined() ? of.second : at::zeros_like(b);
         }
@@ -1233,10 +1256,12 @@ struct Linear : torch::autograd::Function<Linear> {
             if (need_b) out[2] = got[next++];
             return out;
         }
-        const Tensor grad = grads[0].contiguous();
-        if (need_x) out[0] = linear_backward_input(grad, slope, w.contiguous(), Tensor());
+        Tensor grad = grads[0].contiguous(), d = slope;
+        const Activation f{static_cast<int32_t>(ctx->saved_data["kind"].toInt()), ctx->saved_data["scale"].toDouble()};
+        if (need_x && need_w) scale_gradient(grad, d, x, w, f);
+        if (need_x) out[0] = linear_backward_input(grad, d, w.contiguous(), Tensor(), f);
         if (need_w || need_b) {
-            std::tie(out[1], out[2]) = linear_backward_weight({grad, slope, readable(x)}, {}, false, need_w, need_b);
+            std::tie(out[1], out[2]) = linear_backward_weight({grad, d, readable(x)}, {}, false, need_w, need_b, f);
         }
         return out;
     }

@@ -473,6 +473,18 @@ int run_norm(NormKind kind, const ash_norm_args* args, void* stream, const char*
 // ------------------------------------------------------------------- dense layers
 constexpr int64_t kMaxFeatures = 65536;
 
+// grad * slope, rounded to the operands' type as the products round it.
+template <typename T, typename S>
+__global__ __launch_bounds__(kThreads) void scale_kernel(const T* grad, const S* slope, float factor, T* out, int64_t n) {
+    const int64_t at = (static_cast<int64_t>(blockIdx.x) * kThreads + threadIdx.x) * 8;
+    float g[8], d[8];
+    read8(grad + at, n - at, g);
+    read8(slope + at, n - at, d);
+#pragma unroll
+    for (int i = 0; i < 8; ++i) g[i] *= factor * d[i];
+    write8(out + at, n - at, g);
+}
+
 int run_linear(LinearKind kind, const LinearJob& j, int32_t dtype, hipStream_t s) {
     switch (dtype) {
         case ASH_F32: return linear_run<ASH_F32>(kind, j, s);
@@ -525,18 +537,20 @@ LinearJob job_of(const ash_linear_args& a) {
     j.activation = a.activation;
     j.act_scale = a.activation_scale;
     j.splits = 1;
+    j.slope_factor = a.activation == ASH_ACT_SINE ? a.activation_scale : 1.0f;
     return j;
 }
 
 }  // namespace
 
-// Enough workgroups for two a CU, parts of four steps of k at least.
+// Enough workgroups for two a CU (one of the largest tiles), parts of four steps of k at
+// least.
 int32_t linear_splits(int64_t rows, int64_t in, int64_t out, int32_t dtype, int pairs) {
-    const bool narrow = dtype == ASH_F32;
-    const int64_t row_tile = out <= 64 ? 64 : 128, col_tile = in <= 32 ? 32 : (narrow || in <= 64 || out <= 64) ? 64 : 128;
-    const int64_t tiles = ((out + row_tile - 1) / row_tile) * ((in + col_tile - 1) / col_tile) * pairs;
-    const int64_t steps = (rows + (narrow ? 31 : 63)) / (narrow ? 32 : 64);
-    const int64_t wanted = (512 + tiles - 1) / tiles, most = steps / 4 > 0 ? steps / 4 : 1;
+    const WeightTile t = weight_tile(in, out, dtype);
+    const int64_t tiles = ((out + t.rows - 1) / t.rows) * ((in + t.cols - 1) / t.cols) * pairs;
+    const int64_t step = dtype == ASH_F32 ? 32 : 64, steps = (rows + step - 1) / step;
+    const int64_t groups = t.rows == 256 ? 256 : 512;
+    const int64_t wanted = (groups + tiles - 1) / tiles, most = steps / 4 > 0 ? steps / 4 : 1;
     return static_cast<int32_t>(wanted < most ? wanted : most);
 }
 
@@ -575,6 +589,37 @@ int ash_linear_backward_input(const ash_linear_args* args, const void* grad, con
     PointerGuard guard;
     ASH_HIP(guard.enter_for(grad));
     return run_linear(kLinearGradInput, j, args->dtype, static_cast<hipStream_t>(stream));
+}
+
+int ash_linear_wants_scaled_gradient(int64_t rows, int64_t in_features, int64_t out_features, int32_t dtype) {
+    return (dtype == ASH_BF16 || dtype == ASH_F16) && rows >= 4096 && in_features % 8 == 0 && out_features % 8 == 0 &&
+           weight_tile(in_features, out_features, dtype).rows == 256;
+}
+
+int ash_linear_scale_gradient(const ash_linear_args* args, const void* grad, const void* slope, void* scaled,
+                              void* stream) {
+    if (check_linear(args, false, "linear_scale_gradient") != 0) return 1;
+    if (args->rows == 0) return 0;
+    if (grad == nullptr || slope == nullptr || scaled == nullptr) ASH_FAIL("null pointer in linear_scale_gradient");
+    const int64_t n = args->rows * args->out_features, groups = (n + kThreads * 8 - 1) / (kThreads * 8);
+    if (groups > 0x7FFFFFFFll) ASH_FAIL("linear_scale_gradient: too many rows");
+    const float factor = job_of(*args).slope_factor;
+    PointerGuard guard;
+    ASH_HIP(guard.enter_for(grad));
+    hipStream_t s = static_cast<hipStream_t>(stream);
+    const unsigned grid = static_cast<unsigned>(groups);
+    if (args->dtype == ASH_F32) {
+        scale_kernel<<<grid, kThreads, 0, s>>>(static_cast<const float*>(grad), static_cast<const float*>(slope), factor,
+                                               static_cast<float*>(scaled), n);
+    } else if (args->dtype == ASH_BF16) {
+        scale_kernel<<<grid, kThreads, 0, s>>>(static_cast<const __bf16*>(grad), static_cast<const _Float16*>(slope),
+                                               factor, static_cast<__bf16*>(scaled), n);
+    } else {
+        scale_kernel<<<grid, kThreads, 0, s>>>(static_cast<const _Float16*>(grad), static_cast<const float*>(slope),
+                                               factor, static_cast<_Float16*>(scaled), n);
+    }
+    ASH_LAUNCH_CHECK();
+    return 0;
 }
 
 int64_t ash_linear_backward_weight_scratch_bytes(int64_t rows, int64_t in_features, int64_t out_features,

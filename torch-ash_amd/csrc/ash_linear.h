@@ -19,7 +19,8 @@ struct LinearJob {
     const void* bias;
     const void* residual;
     const void* grad;         // gradients only: of the output
-    const void* slope;        // f'(z) as the forward left it, or null: one
+    const void* slope;        // f'(z) / slope_factor as the forward left it, or null: one
+    float slope_factor;
     const float* input_scales;
     const float* weight_scales;
     void* out;
@@ -50,6 +51,18 @@ enum LinearKind { kLinearForward, kLinearGradInput, kLinearGradWeight, kLinearSe
 // Defined in ash_linear.hip, one set for every type.
 template <int DTYPE>
 int linear_run(LinearKind kind, const LinearJob& job, hipStream_t s);
+
+// The tile of a weight's gradient (out x in).
+struct WeightTile {
+    int rows, cols;
+};
+inline WeightTile weight_tile(int64_t in, int64_t out, int32_t dtype) {
+    if (in <= 32) return {128, 32};
+    if (out <= 64) return {64, 64};
+    if (dtype == ASH_F32 || in <= 64) return {128, 64};
+    if (in > 512 && out > 512) return {256, 256};
+    return {128, 128};
+}
 
 // Parts that the rows are cut into for a weight's gradient (ash_layers.hip).
 int32_t linear_splits(int64_t rows, int64_t in, int64_t out, int32_t dtype, int pairs);

@@ -60,9 +60,9 @@ template <typename T> struct Form {
     static constexpr int kLane = kIsByte ? 32 : 8;                  // values of k a lane gives to one instruction
     static constexpr int kInner = kStep / (4 * kLane);              // instructions along k a step
     using Unit = std::conditional_t<kScaled, __bf16, T>;            // what two bytes of a chunk hold
+    using Slope = std::conditional_t<std::is_same<T, __bf16>::value, _Float16, float>;   // see activate
 };
 
-constexpr int kThreads = 256;
 
 // Byte at which chunk `c` of row `row` lies in a plane whose rows are RB bytes.  Chunks
 // are exchanged within a line of 128 bytes such that eight lanes that read one chunk of
@@ -79,6 +79,14 @@ __device__ inline int place(int row, int c) {
         const int f = ((line >> 1) & 1) | (((line ^ (line >> 2)) & 1) << 1) | (((line >> 3) & 1) << 2);
         return line * 128 + (((((row & 1) << 2) | c) ^ f) << 4);
     }
+}
+
+// The same for rows of k of ROWS values of two bytes, such that the sixteen lanes that are
+// served together by a turning read (four rows of k, 32 bytes of each) meet different banks.
+template <int ROWS>
+__device__ inline int stacked_place(int k, int c) {
+    if constexpr (ROWS >= 64) return k * ROWS * 2 + ((c ^ ((k & 3) << 1)) << 4);
+    else return k * ROWS * 2 + ((c ^ (k & 2)) << 4);
 }
 
 template <typename T> __device__ inline float as_float(T v) { return static_cast<float>(v); }
@@ -126,9 +134,10 @@ __device__ inline Three split(const float (&v)[8]) {
 // One operand as a kernel gets it.
 struct Side {
     const void* p;
-    const void* mul;    // of the same layout, or null
+    const void* mul;    // of the same layout (in the type of slopes), or null
     int64_t stride;     // values between rows (lying along k) or between values of k
     int64_t rows;
+    float factor;       // of mul
 };
 
 template <typename T> __device__ inline uint4 packed(const float (&v)[8]) {
@@ -159,17 +168,20 @@ __device__ inline void put(char* plane, int row, int chunk, const float (&v)[8])
 }
 
 // Operand that lies along k: row r at p + r * stride.
-template <typename T, int ROWS, bool MUL>
+template <typename T, int ROWS, bool MUL, int THREADS>
 struct Along {
+    using M = typename Form<T>::Slope;
     static constexpr int kChunks = Form<T>::kStep / Form<T>::kChunk;
-    static constexpr int kEach = (ROWS * kChunks + kThreads - 1) / kThreads;
+    static constexpr int kEach = (ROWS * kChunks + THREADS - 1) / THREADS;
     static constexpr int N = Form<T>::kChunk;
-    static_assert(ROWS * kChunks % kThreads == 0 || kEach == 1, "");
+    static_assert(ROWS * kChunks % THREADS == 0 || kEach == 1, "");
     const T* p[kEach];
-    const T* m[kEach];
+    const M* m[kEach];
     int row[kEach], chunk;
     bool mul;
-    Values<T, N> v[kEach], w[kEach];
+    float factor;
+    Values<T, N> v[kEach];
+    Values<M, N> w[kEach];
 
     // kHalves: rows ROWS / 2 and beyond are rows of another operand of the same shape, zeros
     // where there is none (second order)
@@ -177,9 +189,10 @@ struct Along {
     __device__ void start(const Side& a, int64_t row0, const void* other, int64_t other_stride) {
         chunk = threadIdx.x % kChunks;
         mul = MUL && a.mul != nullptr;
+        factor = a.factor;
 #pragma unroll
         for (int i = 0; i < kEach; ++i) {
-            row[i] = (threadIdx.x + i * kThreads) / kChunks;
+            row[i] = (threadIdx.x + i * THREADS) / kChunks;
             int r = row[i];
             const T* base = static_cast<const T*>(a.p);
             int64_t stride = a.stride;
@@ -190,7 +203,7 @@ struct Along {
             }
             const bool there = base != nullptr && row[i] < ROWS && row0 + r < a.rows;
             p[i] = there ? base + (row0 + r) * stride : nullptr;
-            if constexpr (MUL) m[i] = there && mul ? static_cast<const T*>(a.mul) + (row0 + r) * stride : nullptr;
+            if constexpr (MUL) m[i] = there && mul ? static_cast<const M*>(a.mul) + (row0 + r) * stride : nullptr;
         }
     }
     __device__ void load(int64_t k0, int64_t k_end) {
@@ -200,13 +213,13 @@ struct Along {
             const int64_t left = p[i] != nullptr ? k_end - k : 0;
             v[i] = read<T, N>(p[i] + k, left);
             if constexpr (MUL) {
-                if (mul) w[i] = read<T, N>(m[i] + k, left);
+                if (mul) w[i] = read<M, N>(m[i] + k, left);
             }
         }
     }
     __device__ void store(char* plane) {
         constexpr int RB = kChunks * 16;
-        if (ROWS * kChunks < kThreads && row[0] >= ROWS) return;
+        if (ROWS * kChunks < THREADS && row[0] >= ROWS) return;
 #pragma unroll
         for (int i = 0; i < kEach; ++i) {
             if constexpr (Form<T>::kParts == 3 || MUL || (Form<T>::kScaled && !Form<T>::kIsByte)) {
@@ -216,7 +229,7 @@ struct Along {
                 if constexpr (MUL) {
                     if (mul) {
 #pragma unroll
-                        for (int j = 0; j < 8; ++j) f[j] *= as_float(w[i].v[j]);
+                        for (int j = 0; j < 8; ++j) f[j] *= factor * as_float(w[i].v[j]);
                     }
                 }
                 put<T, ROWS>(plane, row[i], chunk, f);
@@ -229,19 +242,21 @@ struct Along {
     }
 };
 
-// Operand that lies across k: value k of row r at p[k * stride + r].  A thread takes
-// eight values of k of kWide consecutive rows and turns them.
-template <typename T, int ROWS, bool MUL>
+// Operand that lies across k, float32: value k of row r at p[k * stride + r].  A thread
+// takes eight values of k of kWide consecutive rows and turns them.
+template <typename T, int ROWS, bool MUL, int THREADS>
 struct Across {
     static constexpr int kGroups = Form<T>::kStep / 8;
-    static constexpr int kWide = ROWS * kGroups >= kThreads ? ROWS * kGroups / kThreads : 1;
+    static constexpr int kWide = ROWS * kGroups >= THREADS ? ROWS * kGroups / THREADS : 1;
     static constexpr int kUnits = ROWS / kWide * kGroups;
     const T* p;
-    const T* m;
+    const typename Form<T>::Slope* m;
     int64_t stride, left;   // rows from this thread's first to the last
     int row, group;
     bool mul, works;
-    Values<T, kWide> v[8], w[8];
+    float factor;
+    Values<T, kWide> v[8];
+    Values<typename Form<T>::Slope, kWide> w[8];
 
     template <bool>
     __device__ void start(const Side& a, int64_t row0, const void*, int64_t) {
@@ -252,7 +267,8 @@ struct Across {
         left = works ? a.rows - (row0 + row) : 0;
         mul = MUL && a.mul != nullptr;
         p = static_cast<const T*>(a.p) + row0 + row;
-        m = mul ? static_cast<const T*>(a.mul) + row0 + row : nullptr;
+        factor = a.factor;
+        m = mul ? static_cast<const typename Form<T>::Slope*>(a.mul) + row0 + row : nullptr;
     }
     __device__ void load(int64_t k0, int64_t k_end) {
 #pragma unroll
@@ -261,7 +277,7 @@ struct Across {
             const int64_t n = k < k_end ? left : 0;
             v[j] = read<T, kWide>(p + k * stride, n);
             if constexpr (MUL) {
-                if (mul) w[j] = read<T, kWide>(m + k * stride, n);
+                if (mul) w[j] = read<typename Form<T>::Slope, kWide>(m + k * stride, n);
             }
         }
     }
@@ -274,10 +290,67 @@ struct Across {
             for (int j = 0; j < 8; ++j) {
                 f[j] = as_float(v[j].v[i]);
                 if constexpr (MUL) {
-                    if (mul) f[j] *= as_float(w[j].v[i]);
+                    if (mul) f[j] *= factor * as_float(w[j].v[i]);
                 }
             }
             put<T, ROWS>(plane, row + i, group, f);
+        }
+    }
+};
+
+// Operand that lies across k, two bytes a value: rows of k go into LDS as they are, and the
+// reads turn them (fetch_stacked).
+template <typename T, int ROWS, bool MUL, int THREADS>
+struct Stacked {
+    using M = typename Form<T>::Slope;
+    static constexpr int kChunks = ROWS / 8;
+    static constexpr int kEach = Form<T>::kStep * kChunks / THREADS;
+    static_assert(Form<T>::kStep * kChunks % THREADS == 0, "");
+    const T* p;
+    const M* m;
+    int64_t stride, left;
+    int chunk;
+    bool mul;
+    float factor;
+    Values<T, 8> v[kEach];
+    Values<M, 8> w[kEach];
+
+    template <bool>
+    __device__ void start(const Side& a, int64_t row0, const void*, int64_t) {
+        chunk = threadIdx.x % kChunks;
+        stride = a.stride;
+        left = a.rows - (row0 + chunk * 8);
+        mul = MUL && a.mul != nullptr;
+        factor = a.factor;
+        p = static_cast<const T*>(a.p) + row0 + chunk * 8;
+        m = mul ? static_cast<const M*>(a.mul) + row0 + chunk * 8 : nullptr;
+    }
+    __device__ int row(int i) const { return (threadIdx.x + i * THREADS) / kChunks; }
+    __device__ void load(int64_t k0, int64_t k_end) {
+#pragma unroll
+        for (int i = 0; i < kEach; ++i) {
+            const int64_t k = k0 + row(i);
+            const int64_t n = k < k_end ? left : 0;
+            v[i] = read<T, 8>(p + k * stride, n);
+            if constexpr (MUL) {
+                if (mul) w[i] = read<M, 8>(m + k * stride, n);
+            }
+        }
+    }
+    __device__ void store(char* plane) {
+#pragma unroll
+        for (int i = 0; i < kEach; ++i) {
+            uint4 u;
+            __builtin_memcpy(&u, &v[i], 16);
+            if constexpr (MUL) {
+                if (mul) {
+                    float f[8];
+#pragma unroll
+                    for (int j = 0; j < 8; ++j) f[j] = as_float(v[i].v[j]) * (factor * as_float(w[i].v[j]));
+                    u = packed<T>(f);
+                }
+            }
+            *reinterpret_cast<uint4*>(plane + stacked_place<ROWS>(row(i), chunk)) = u;
         }
     }
 };
@@ -312,6 +385,25 @@ __device__ inline Fragment<T> fetch(const char* plane, int row0, int inner) {
     return f;
 }
 
+typedef short i16x4 __attribute__((ext_vector_type(4)));
+// Of an operand whose rows of k are stacked: a read of four rows of k by sixteen lanes gives
+// lane i the four values of column i.
+template <typename T, int ROWS>
+__device__ inline Fragment<T> fetch_stacked(char* plane, int row0, int inner) {
+    const int lane = threadIdx.x & 63, i = lane & 15;
+    const int k = inner * 32 + (lane >> 4) * 8 + (i >> 2), row = row0 + (i & 3) * 4;
+    char* at = plane + stacked_place<ROWS>(k, row >> 3) + (row & 7) * 2;
+    i16x4 half[2];
+#pragma unroll
+    for (int h = 0; h < 2; ++h) {
+        half[h] = __builtin_amdgcn_ds_read_tr16_b64_v4i16(
+                (__attribute__((address_space(3))) i16x4*)(at + h * 4 * ROWS * 2));
+    }
+    Fragment<T> f;
+    __builtin_memcpy(&f.v, half, 16);
+    return f;
+}
+
 __device__ inline f32x4 mma(const Fragment<__bf16>& q, const Fragment<__bf16>& p, f32x4 c) {
     return __builtin_amdgcn_mfma_f32_16x16x32_bf16(q.v, p.v, c, 0, 0, 0);
 }
@@ -335,6 +427,7 @@ __device__ inline f32x4 mma(const Fragment<E4M3>& q, const Fragment<E4M3>& p, f3
     return __builtin_amdgcn_mfma_scale_f32_16x16x128_f8f6f4(q.v, p.v, c, 0, 0, 0, 0x7F7F7F7F, 0, 0x7F7F7F7F);
 }
 // Row sums of P (every row of the result is the same): the bias' gradient.
+__device__ inline f32x4 sum_rows(const Fragment<E4M3>&, f32x4 c) { return c; }   // 8-bit rows have none
 __device__ inline f32x4 sum_rows(const Fragment<__bf16>& p, f32x4 c) {
     const bf16x8 one = {1.0f, 1.0f, 1.0f, 1.0f, 1.0f, 1.0f, 1.0f, 1.0f};
     return __builtin_amdgcn_mfma_f32_16x16x32_bf16(one, p.v, c, 0, 0, 0);
@@ -352,7 +445,10 @@ __device__ inline f32x4 sum_rows(const Fragment<float>& p, f32x4 c) {
 // --------------------------------------------------------------------- activations
 __device__ inline float sigmoid(float v) { return 1.0f / (1.0f + expf(-v)); }
 
-// f(z), f'(z) and f''(z) of eight values at a time.
+// Slopes that are kept for a backward pass are float32, for bf16 operands fp16: a rounding
+// of them to the operands' type would be one more of the size of that of gz and of the
+// result (half as much again in the gradients' error).  That of a sine is kept without the
+// factor a, so that all fit fp16 (they are at most 1.13).
 template <int N>
 __device__ inline void activate(int kind, float a, const float (&z)[N], float (&y)[N], float (&d)[N]) {
     switch (kind) {
@@ -395,7 +491,7 @@ __device__ inline void activate(int kind, float a, const float (&z)[N], float (&
                 float s, c;
                 sincosf(a * z[i], &s, &c);
                 y[i] = s;
-                d[i] = a * c;
+                d[i] = c;
             }
             break;
         default:
@@ -513,64 +609,213 @@ __device__ inline void banded(const Product& a, int64_t tile, int64_t& row, int6
     col = in_band / rows;
 }
 
+// How a tile is shared out among wavefronts, and how much of it passes through LDS at a time
+// on its way out.
+template <int BR, int BC>
+struct Tile {
+    static constexpr int kThreads = BR * BC >= 256 * 256 ? 512 : 256, kWaves = kThreads / 64;
+    static constexpr int kWaveCols = BC >= 256 ? 4 : BC >= 128 ? 2 : BR >= 128 ? 1 : 2;
+    static constexpr int kWaveRows = kWaves / kWaveCols;
+    static constexpr int kR = BR / kWaveRows / 16, kC = BC / kWaveCols / 16;
+    static constexpr int kSums = kR / kWaveCols;   // rows of P are summed by those that share them, so many of kR each
+    static constexpr int kPass = kR > 4 ? 2 : kR, kPasses = kR / kPass;   // of kR
+    static constexpr int kOutRows = kWaveRows * kPass * 16;
+};
+
 template <typename T, int BR, int BC> struct Shared {
     static constexpr int kRowBytes = Form<T>::kStep / Form<T>::kChunk * 16;
     static constexpr int kP = Form<T>::kParts * BR * kRowBytes;
     static constexpr int kQ = Form<T>::kParts * BC * kRowBytes;
     static constexpr int kStride = BC + 4;       // floats between rows of the result
-    static constexpr int kOut = BR * kStride * 4;
+    static constexpr int kOut = Tile<BR, BC>::kOutRows * kStride * 4;
     static constexpr int kBytes = 2 * (kP + kQ) > kOut ? 2 * (kP + kQ) : kOut;
 };
 
-template <typename T, int BR, int BC>
-struct Tile {
-    static constexpr int kWaveCols = BC >= 128 ? 2 : (BR >= 128 ? 1 : 2);
-    static constexpr int kWaveRows = 4 / kWaveCols;
-    static constexpr int kR = BR / kWaveRows / 16, kC = BC / kWaveCols / 16;
-};
+// The way out of a tile's sums.  They go through LDS once more, so that a thread has eight
+// columns of a row: operands and results then come and go in whole lines.
+template <typename T, typename TO, int BR, int BC, int KIND, int PASS>
+__device__ inline void finish_pass(const Product& a, char* lds, const f32x4 (&acc)[Tile<BR, BC>::kR][Tile<BR, BC>::kC],
+                                   int64_t row0, int64_t col0, const float (&bias)[8], const float (&scale)[8]) {
+    using W = Tile<BR, BC>;
+    constexpr int kStride = Shared<T, BR, BC>::kStride;
+    constexpr int kAcross = BC / 8, kDown = W::kThreads / kAcross;
+    constexpr int kPassRows = KIND == kLinearSecond ? W::kOutRows / 2 : W::kOutRows;
+    const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+    const int wave_col = wave % W::kWaveCols * W::kC * 16;
+    float* sums_of = reinterpret_cast<float*>(lds);
+    __syncthreads();
+#pragma unroll
+    for (int r = 0; r < W::kPass; ++r) {
+#pragma unroll
+        for (int c = 0; c < W::kC; ++c) {
+            *reinterpret_cast<f32x4*>(sums_of + ((wave / W::kWaveCols * W::kPass + r) * 16 + (lane & 15)) * kStride +
+                                      wave_col + c * 16 + (lane >> 4) * 4) = acc[PASS * W::kPass + r][c];
+        }
+    }
+    __syncthreads();
+    const LinearJob& j = a.job;
+    const int at = threadIdx.x % kAcross * 8;
+    const int64_t col = col0 + at, left = a.q.rows - col;
+#pragma unroll 1
+    for (int r = threadIdx.x / kAcross; r < kPassRows; r += kDown) {
+        // rows 16 kPass w and on of a pass are those of the wavefronts' row w
+        const int64_t row = row0 + r / (W::kPass * 16) * W::kR * 16 + PASS * W::kPass * 16 + r % (W::kPass * 16);
+        if (row >= a.p.rows || left <= 0) continue;
+        float z[8], y[8], d[8];
+        const float row_scale = Form<T>::kScaled ? j.input_scales[row] : 1.0f;
+#pragma unroll
+        for (int i = 0; i < 8; ++i) {
+            z[i] = sums_of[r * kStride + at + i];
+            if constexpr (Form<T>::kScaled) z[i] *= row_scale * scale[i];
+            z[i] += bias[i];
+        }
+        const int64_t o = row * a.q.rows + col;
+        if constexpr (KIND == kLinearSecond) {
+            // t: the derivative of <second input, gradient of the input> by gz
+            float t[8], g[8], dd[8];
+#pragma unroll
+            for (int i = 0; i < 8; ++i) t[i] = sums_of[(kPassRows + r) * kStride + at + i];
+            if (j.addend != nullptr) {
+                float more[8];
+                read8(static_cast<const TO*>(j.addend) + row * j.addend_stride + col, left, more);
+#pragma unroll
+                for (int i = 0; i < 8; ++i) t[i] += more[i];
+            }
+            read8(static_cast<const TO*>(j.grad) + o, left, g);
+            curve(j.activation, j.act_scale, z, d, dd);
+#pragma unroll
+            for (int i = 0; i < 8; ++i) {
+                y[i] = t[i] * d[i];
+                dd[i] *= t[i] * g[i];
+            }
+            if (j.out != nullptr) write8(static_cast<TO*>(j.out) + o, left, y);
+            if (j.curvature_out != nullptr) write8(static_cast<TO*>(j.curvature_out) + o, left, dd);
+        } else {
+            activate(j.activation, j.act_scale, z, y, d);
+            if (j.residual != nullptr) {
+                float more[8];
+                read8(static_cast<const TO*>(j.residual) + row * j.residual_stride + col, left, more);
+#pragma unroll
+                for (int i = 0; i < 8; ++i) y[i] += more[i];
+            }
+            write8(static_cast<TO*>(j.out) + o, left, y);
+            if (j.slope_out != nullptr) write8(static_cast<typename Form<TO>::Slope*>(j.slope_out) + o, left, d);
+        }
+    }
+    if constexpr (PASS + 1 < W::kPasses) {
+        finish_pass<T, TO, BR, BC, KIND, PASS + 1>(a, lds, acc, row0, col0, bias, scale);
+    }
+}
 
 template <typename T, typename TO, int BR, int BC, int KIND>
-__global__ __launch_bounds__(kThreads) void product_kernel(const Product a) {
+__device__ inline void finish(const Product& a, char* lds, const f32x4 (&acc)[Tile<BR, BC>::kR][Tile<BR, BC>::kC],
+                              int64_t row0, int64_t col0) {
+    const int64_t col = col0 + threadIdx.x % (BC / 8) * 8, left = a.q.rows - col;
+    float bias[8], scale[8];
+#pragma unroll
+    for (int i = 0; i < 8; ++i) {
+        bias[i] = 0.0f;
+        scale[i] = 1.0f;
+    }
+    if (a.job.bias != nullptr) read8(static_cast<const TO*>(a.job.bias) + col, left, bias);
+    if constexpr (Form<T>::kScaled) read8(a.job.weight_scales + col, left, scale);
+    finish_pass<T, TO, BR, BC, KIND, 0>(a, lds, acc, row0, col0, bias, scale);
+}
+
+// A part's sums of a weight's gradient, in float32; join_kernel joins the parts.
+template <int BR, int BC>
+__device__ inline void leave_part(const Product& a, const f32x4 (&acc)[Tile<BR, BC>::kR][Tile<BR, BC>::kC],
+                                  const f32x4 (&rows_sum)[Tile<BR, BC>::kSums], int64_t part, int64_t row0, int64_t col0,
+                                  bool sums) {
+    using W = Tile<BR, BC>;
+    const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+    const int wave_row = wave / W::kWaveCols * W::kR * 16, wave_col = wave % W::kWaveCols * W::kC * 16;
+    float* out = static_cast<float*>(a.job.scratch) + part * (a.p.rows * a.q.rows + a.p.rows);
+    float* bias = out + a.p.rows * a.q.rows;
+#pragma unroll
+    for (int r = 0; r < W::kR; ++r) {
+        const int64_t row = row0 + wave_row + r * 16 + (lane & 15);
+        if (row >= a.p.rows) continue;
+#pragma unroll
+        for (int c = 0; c < W::kC; ++c) {
+            const int64_t col = col0 + wave_col + c * 16 + (lane >> 4) * 4;
+            float* at = out + row * a.q.rows + col;
+            if (col + 4 <= a.q.rows) {
+                __builtin_memcpy(at, &acc[r][c], 16);
+            } else {
+#pragma unroll
+                for (int i = 0; i < 4; ++i) {
+                    if (col + i < a.q.rows) at[i] = acc[r][c][i];
+                }
+            }
+        }
+        if (sums && r / W::kSums == wave % W::kWaveCols && lane < 16) bias[row] = rows_sum[r % W::kSums][0];
+    }
+}
+
+// The tile of a workgroup: what it computes (of a weight's gradient, which part of k too).
+struct Place {
+    int64_t row_tile, col_tile, part, k0, k_end;
+    bool second, sums;
+};
+template <int KIND> __device__ inline bool place_of(const Product& a, Place& w) {
+    const int64_t tiles = a.row_tiles * a.col_tiles;
+    int64_t tile;
+    if (!tile_of(a, tiles * (KIND == kLinearGradWeight ? a.parts * a.pairs : 1), tile)) return false;
+    w.part = 0;
+    w.k0 = 0;
+    w.k_end = a.k;
+    w.second = w.sums = false;
+    if constexpr (KIND == kLinearGradWeight) {
+        w.part = tile / tiles;
+        tile = tile % tiles;
+        w.second = w.part >= a.parts;
+        w.k0 = (w.second ? w.part - a.parts : w.part) * a.part_rows;
+        w.k_end = w.k0 + a.part_rows < a.k ? w.k0 + a.part_rows : a.k;
+        w.row_tile = tile % a.row_tiles;
+        w.col_tile = tile / a.row_tiles;
+        w.sums = a.job.bias_out != nullptr && w.col_tile == 0 && w.second == a.second_has_bias;
+    } else {
+        banded(a, tile, w.row_tile, w.col_tile);
+    }
+    return true;
+}
+
+template <typename T, typename TO, int BR, int BC, int KIND>
+__global__ __launch_bounds__((Tile<BR, BC>::kThreads)) void product_kernel(const Product a) {
     using S = Shared<T, BR, BC>;
-    using W = Tile<T, BR, BC>;
+    using W = Tile<BR, BC>;
+    constexpr int kThreads = W::kThreads;
     constexpr bool kGrad = KIND == kLinearGradInput || KIND == kLinearGradWeight;
     constexpr int kStep = Form<T>::kStep;
     __shared__ __attribute__((aligned(16))) char lds[S::kBytes];
 
-    const int64_t tiles = a.row_tiles * a.col_tiles;
-    int64_t tile, row_tile, col_tile;
-    if (!tile_of(a, tiles * (KIND == kLinearGradWeight ? a.parts * a.pairs : 1), tile)) return;
-    int64_t k0 = 0, k_end = a.k;
-    bool second = false, sums = false;
-    int64_t part = 0;
-    if constexpr (KIND == kLinearGradWeight) {
-        part = tile / tiles;
-        tile = tile % tiles;
-        second = part >= a.parts;
-        k0 = (second ? part - a.parts : part) * a.part_rows;
-        k_end = k0 + a.part_rows < a.k ? k0 + a.part_rows : a.k;
-        row_tile = tile % a.row_tiles;
-        col_tile = tile / a.row_tiles;
-        sums = a.job.bias_out != nullptr && col_tile == 0 && second == a.second_has_bias;
-    } else {
-        banded(a, tile, row_tile, col_tile);
-    }
-    constexpr int kRowsOut = KIND == kLinearSecond ? BR / 2 : BR;
-    const int64_t row0 = row_tile * kRowsOut, col0 = col_tile * BC;
+    Place w;
+    if (!place_of<KIND>(a, w)) return;
+    const int64_t k0 = w.k0, k_end = w.k_end;
+    const int64_t row0 = w.row_tile * (KIND == kLinearSecond ? BR / 2 : BR), col0 = w.col_tile * BC;
 
-    using LoadP = std::conditional_t<KIND == kLinearGradWeight, Across<T, BR, true>, Along<T, BR, kGrad>>;
-    using LoadQ = std::conditional_t<kGrad, Across<T, BC, false>, Along<T, BC, false>>;
+    constexpr bool kStackP = KIND == kLinearGradWeight && sizeof(T) == 2, kStackQ = kGrad && sizeof(T) == 2;
+    using LoadP = std::conditional_t<kStackP, Stacked<T, BR, true, kThreads>,
+                                     std::conditional_t<KIND == kLinearGradWeight, Across<T, BR, true, kThreads>,
+                                                        Along<T, BR, kGrad, kThreads>>>;
+    using LoadQ = std::conditional_t<kStackQ, Stacked<T, BC, false, kThreads>,
+                                     std::conditional_t<kGrad, Across<T, BC, false, kThreads>,
+                                                        Along<T, BC, false, kThreads>>>;
     LoadP p;
     LoadQ q;
-    p.template start<KIND == kLinearSecond>(second ? a.p2 : a.p, row0, a.other, a.other_stride);
-    q.template start<false>(second ? a.q2 : a.q, col0, nullptr, 0);
+    p.template start<KIND == kLinearSecond>(w.second ? a.p2 : a.p, row0, a.other, a.other_stride);
+    q.template start<false>(w.second ? a.q2 : a.q, col0, nullptr, 0);
 
-    const int wave = threadIdx.x >> 6;
+    // (matrix instructions do not go by the mask of lanes: what they depend on has to be known
+    // to be the same for a wavefront)
+    const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
     const int wave_row = wave / W::kWaveCols * W::kR * 16, wave_col = wave % W::kWaveCols * W::kC * 16;
-    f32x4 acc[W::kR][W::kC], rows_sum[W::kR];
+    f32x4 acc[W::kR][W::kC], rows_sum[W::kSums];
+#pragma unroll
+    for (int r = 0; r < W::kSums; ++r) rows_sum[r] = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
 #pragma unroll
     for (int r = 0; r < W::kR; ++r) {
-        rows_sum[r] = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
 #pragma unroll
         for (int c = 0; c < W::kC; ++c) acc[r][c] = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
     }
@@ -596,14 +841,21 @@ __global__ __launch_bounds__(kThreads) void product_kernel(const Product a) {
             if (Form<T>::kInner > 1 && k + inner * (kStep / Form<T>::kInner) >= k_end) break;
             Fragment<T> fq[W::kC];
 #pragma unroll
-            for (int c = 0; c < W::kC; ++c) fq[c] = fetch<T, BC>(now + S::kP, wave_col + c * 16, inner);
+            for (int c = 0; c < W::kC; ++c) {
+                if constexpr (kStackQ) fq[c] = fetch_stacked<T, BC>(now + S::kP, wave_col + c * 16, inner);
+                else fq[c] = fetch<T, BC>(now + S::kP, wave_col + c * 16, inner);
+            }
 #pragma unroll
             for (int r = 0; r < W::kR; ++r) {
-                const Fragment<T> fp = fetch<T, BR>(now, wave_row + r * 16, inner);
+                Fragment<T> fp;
+                if constexpr (kStackP) fp = fetch_stacked<T, BR>(now, wave_row + r * 16, inner);
+                else fp = fetch<T, BR>(now, wave_row + r * 16, inner);
 #pragma unroll
                 for (int c = 0; c < W::kC; ++c) acc[r][c] = mma(fq[c], fp, acc[r][c]);
                 if constexpr (KIND == kLinearGradWeight) {
-                    if (sums) rows_sum[r] = sum_rows(fp, rows_sum[r]);
+                    if (w.sums && r / W::kSums == wave % W::kWaveCols) {
+                        rows_sum[r % W::kSums] = sum_rows(fp, rows_sum[r % W::kSums]);
+                    }
                 }
             }
         }
@@ -613,98 +865,202 @@ __global__ __launch_bounds__(kThreads) void product_kernel(const Product a) {
         }
     }
 
-    const int lane = threadIdx.x & 63;
     if constexpr (KIND == kLinearGradWeight) {
-        // a part's sums, in float32; reduce_kernel joins the parts
-        float* out = static_cast<float*>(a.job.scratch) + part * (a.p.rows * a.q.rows + a.p.rows);
-        float* bias = out + a.p.rows * a.q.rows;
-#pragma unroll
-        for (int r = 0; r < W::kR; ++r) {
-            const int64_t row = row0 + wave_row + r * 16 + (lane & 15);
-            if (row >= a.p.rows) continue;
-#pragma unroll
-            for (int c = 0; c < W::kC; ++c) {
-                const int64_t col = col0 + wave_col + c * 16 + (lane >> 4) * 4;
-#pragma unroll
-                for (int i = 0; i < 4; ++i) {
-                    if (col + i < a.q.rows) out[row * a.q.rows + col + i] = acc[r][c][i];
-                }
-            }
-            if (sums && wave_col == 0 && lane < 16) bias[row] = rows_sum[r][0];
-        }
-        return;
+        leave_part<BR, BC>(a, acc, rows_sum, w.part, row0, col0, w.sums);
     } else {
-        // the tile goes through LDS once more, so that a thread has eight columns of a row:
-        // operands and results then come and go in whole lines
-        __syncthreads();
-        float* sums_of = reinterpret_cast<float*>(lds);
-#pragma unroll
-        for (int r = 0; r < W::kR; ++r) {
-#pragma unroll
-            for (int c = 0; c < W::kC; ++c) {
-                *reinterpret_cast<f32x4*>(sums_of + (wave_row + r * 16 + (lane & 15)) * S::kStride + wave_col +
-                                          c * 16 + (lane >> 4) * 4) = acc[r][c];
-            }
+        finish<T, TO, BR, BC, KIND>(a, lds, acc, row0, col0);
+    }
+}
+
+// Large products of operands of one or two bytes: tiles of 256 x 256, whose operands go from
+// memory into LDS without passing through registers, so that a wavefront can hold 128 x 64
+// sums (with 64 x 64 a wavefront the reads from LDS take as long as the products).  Both
+// halves of a step's 16-byte pieces are addressed such that they land where place() and
+// stacked_place() look for them.  Pieces past an operand's end, and past the last k, are
+// outside of the buffer that the loads are told of, and come as zeros.
+constexpr int kLarge = 256, kLargeThreads = 512, kLargeEach = 4;   // pieces a thread, operand and step
+constexpr uint32_t kNowhere = 0x80000000u;                         // beyond every such buffer
+
+template <typename T, bool STACKED>
+struct Direct {
+    const char* base;       // of the tile, at the first k
+    uint32_t offset[kLargeEach], stride;
+    int k_of;               // first k of this thread's pieces along a row
+    int64_t extent;         // bytes from base to the operand's end (of k_end)
+
+    __device__ void start(const Side& a, int64_t row0, int64_t k0, int64_t k_end) {
+        const int64_t rows = a.rows - row0 < kLarge ? a.rows - row0 : kLarge;
+        stride = static_cast<uint32_t>(a.stride * sizeof(T));
+        if constexpr (STACKED) {
+            base = static_cast<const char*>(a.p) + (k0 * a.stride + row0) * sizeof(T);
+            extent = ((k_end - k0 - 1) * a.stride + rows) * sizeof(T);
+        } else {
+            base = static_cast<const char*>(a.p) + (row0 * a.stride + k0) * sizeof(T);
+            extent = ((rows - 1) * a.stride + (k_end - k0)) * sizeof(T);
         }
-        __syncthreads();
-        constexpr int kAcross = BC / 8, kDown = kThreads / kAcross;
-        const LinearJob& j = a.job;
-        const int at = threadIdx.x % kAcross * 8;
-        const int64_t col = col0 + at, left = a.q.rows - col;
-        if (left <= 0) return;
-        float bias[8], scale[8];
+        k_of = 0;
 #pragma unroll
-        for (int i = 0; i < 8; ++i) {
-            bias[i] = 0.0f;
-            scale[i] = 1.0f;
-        }
-        if (j.bias != nullptr) read8(static_cast<const TO*>(j.bias) + col, left, bias);
-        if constexpr (Form<T>::kScaled) read8(j.weight_scales + col, left, scale);
-#pragma unroll 1
-        for (int r = threadIdx.x / kAcross; r < kRowsOut; r += kDown) {
-            const int64_t row = row0 + r;
-            if (row >= a.p.rows) break;
-            float z[8], y[8], d[8];
-            const float row_scale = Form<T>::kScaled ? j.input_scales[row] : 1.0f;
-#pragma unroll
-            for (int i = 0; i < 8; ++i) {
-                z[i] = sums_of[r * S::kStride + at + i];
-                if constexpr (Form<T>::kScaled) z[i] *= row_scale * scale[i];
-                z[i] += bias[i];
-            }
-            const int64_t o = row * a.q.rows + col;
-            if constexpr (KIND == kLinearSecond) {
-                // t: the derivative of <second input, gradient of the input> by gz
-                float t[8], g[8], dd[8];
-#pragma unroll
-                for (int i = 0; i < 8; ++i) t[i] = sums_of[(kRowsOut + r) * S::kStride + at + i];
-                if (j.addend != nullptr) {
-                    float more[8];
-                    read8(static_cast<const TO*>(j.addend) + row * j.addend_stride + col, left, more);
-#pragma unroll
-                    for (int i = 0; i < 8; ++i) t[i] += more[i];
-                }
-                read8(static_cast<const TO*>(j.grad) + o, left, g);
-                curve(j.activation, j.act_scale, z, d, dd);
-#pragma unroll
-                for (int i = 0; i < 8; ++i) {
-                    y[i] = t[i] * d[i];
-                    dd[i] *= t[i] * g[i];
-                }
-                if (j.out != nullptr) write8(static_cast<TO*>(j.out) + o, left, y);
-                if (j.curvature_out != nullptr) write8(static_cast<TO*>(j.curvature_out) + o, left, dd);
+        for (int i = 0; i < kLargeEach; ++i) {
+            const int piece = threadIdx.x + i * kLargeThreads;
+            if constexpr (STACKED) {
+                const int k = piece >> 5, c = (piece & 31) ^ ((k & 3) << 1);
+                offset[i] = k * stride + c * 16;
             } else {
-                activate(j.activation, j.act_scale, z, y, d);
-                if (j.residual != nullptr) {
-                    float more[8];
-                    read8(static_cast<const TO*>(j.residual) + row * j.residual_stride + col, left, more);
-#pragma unroll
-                    for (int i = 0; i < 8; ++i) y[i] += more[i];
-                }
-                write8(static_cast<TO*>(j.out) + o, left, y);
-                if (j.slope_out != nullptr) write8(static_cast<TO*>(j.slope_out) + o, left, d);
+                const int row = piece >> 3, c = (piece & 7) ^ (row & 7);
+                k_of = c * Form<T>::kChunk;
+                offset[i] = row * stride + c * 16;
             }
         }
+    }
+    // `k`: from k0
+    __device__ void issue(char* plane, int k, int k_left) {
+        const int64_t past = STACKED ? static_cast<int64_t>(k) * stride : k * static_cast<int>(sizeof(T));
+        const int64_t left = extent > past ? extent - past : 0;
+        const auto buffer = __builtin_amdgcn_make_buffer_rsrc(
+                const_cast<char*>(base + past), 0, static_cast<int>(left < 0x7FFFFFFF ? left : 0x7FFFFFFF), 0x00020000);
+        const bool there = STACKED || k_of < k_left;
+#pragma unroll
+        for (int i = 0; i < kLargeEach; ++i) {
+            // a wavefront's pieces are consecutive
+            char* at = plane + __builtin_amdgcn_readfirstlane(threadIdx.x >> 6) * 1024 + i * kLargeThreads * 16;
+            __builtin_amdgcn_raw_ptr_buffer_load_lds(
+                    buffer, (__attribute__((address_space(3))) void*)at, 16, there ? offset[i] : kNowhere, 0, 0, 0);
+        }
+    }
+};
+
+// Where a lane's pieces lie: addresses differ from one another by constants (Along), or go
+// round in four (Stacked), so that a wavefront keeps a few of them in registers.
+template <typename T, bool STACKED>
+struct Reader {
+    const char* at[STACKED ? 4 : 2];
+
+    __device__ Reader(const char* plane, int row0) {
+        const int lane = threadIdx.x & 63, i = lane & 15, g = lane >> 4;
+        if constexpr (STACKED) {
+            const int k = g * 8 + (i >> 2);
+#pragma unroll
+            for (int n = 0; n < 4; ++n) {
+                at[n] = plane + k * kLarge * 2 + ((((row0 >> 3) + ((i & 3) >> 1)) ^ (((k & 3) ^ n) << 1)) << 4) + (i & 1) * 8;
+            }
+        } else if constexpr (Form<T>::kIsByte) {
+#pragma unroll
+            for (int n = 0; n < 2; ++n) at[n] = plane + (row0 + i) * 128 + (((2 * g + n) ^ (i & 7)) << 4);
+        } else {
+#pragma unroll
+            for (int n = 0; n < 2; ++n) at[n] = plane + (row0 + i) * 128 + (((4 * n + g) ^ (i & 7)) << 4);
+        }
+    }
+    // rows 16 r and on from row0
+    __device__ Fragment<T> get(int r, int inner) const {
+        Fragment<T> f;
+        if constexpr (STACKED) {
+            i16x4 part[2];
+#pragma unroll
+            for (int h = 0; h < 2; ++h) {
+                const char* p = at[r & 3] + (r >> 2) * 128 + (inner * 32 + h * 4) * kLarge * 2;
+                part[h] = __builtin_amdgcn_ds_read_tr16_b64_v4i16(
+                        (__attribute__((address_space(3))) i16x4*)const_cast<char*>(p));
+            }
+            __builtin_memcpy(&f.v, part, 16);
+        } else if constexpr (Form<T>::kIsByte) {
+            uint4 part[2];
+#pragma unroll
+            for (int n = 0; n < 2; ++n) part[n] = *reinterpret_cast<const uint4*>(at[n] + r * 2048);
+            __builtin_memcpy(&f.v, part, 32);
+        } else {
+            __builtin_memcpy(&f.v, at[inner] + r * 2048, 16);
+        }
+        return f;
+    }
+};
+
+constexpr int kWaitLoads = 0x0F70;   // until no load from memory is under way
+
+template <typename T, typename TO, int KIND>
+__global__ __launch_bounds__(kLargeThreads) void large_kernel(const Product a) {
+    using W = Tile<kLarge, kLarge>;
+    constexpr int kPlane = kLarge * 128, kStep = Form<T>::kStep;
+    constexpr bool kStackP = KIND == kLinearGradWeight, kStackQ = KIND != kLinearForward;
+    static_assert(W::kThreads == kLargeThreads && W::kOutRows * (kLarge + 4) * 4 <= 2 * 2 * kPlane, "");
+    // two halves under names of their own: reads of one need not wait for loads into the other
+    __shared__ __attribute__((aligned(16))) char half0[2 * kPlane];
+    __shared__ __attribute__((aligned(16))) char half1[2 * kPlane];
+
+    Place w;
+    if (!place_of<KIND>(a, w)) return;
+    const int64_t row0 = w.row_tile * kLarge, col0 = w.col_tile * kLarge;
+    const int length = w.k_end > w.k0 ? static_cast<int>(w.k_end - w.k0) : 0;
+    Direct<T, kStackP> p;
+    Direct<T, kStackQ> q;
+    p.start(w.second ? a.p2 : a.p, row0, w.k0, w.k_end);
+    q.start(w.second ? a.q2 : a.q, col0, w.k0, w.k_end);
+
+    // (matrix instructions do not go by the mask of lanes: what they depend on has to be known
+    // to be the same for a wavefront)
+    const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+    const int wave_row = wave / W::kWaveCols * W::kR * 16, wave_col = wave % W::kWaveCols * W::kC * 16;
+    f32x4 acc[W::kR][W::kC], rows_sum[W::kSums];
+#pragma unroll
+    for (int r = 0; r < W::kSums; ++r) rows_sum[r] = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
+#pragma unroll
+    for (int r = 0; r < W::kR; ++r) {
+#pragma unroll
+        for (int c = 0; c < W::kC; ++c) acc[r][c] = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
+    }
+    const auto issue = [&](char* half, int k) {
+        p.issue(half, k, length - k);
+        q.issue(half + kPlane, k, length - k);
+    };
+    const auto arrive = [&] {
+        __builtin_amdgcn_s_waitcnt(kWaitLoads);
+        __syncthreads();   // a step's operands are there, and nobody reads the other half any more
+    };
+    // sums: of P's rows too (by the workgroups that are the first of a row of tiles)
+    const auto run = [&](auto sums) {
+        const Reader<T, kStackP> p0(half0, wave_row), p1(half1, wave_row);
+        const Reader<T, kStackQ> q0(half0 + kPlane, wave_col), q1(half1 + kPlane, wave_col);
+        const auto multiply = [&](const auto& rp, const auto& rq) {
+#pragma unroll
+            for (int inner = 0; inner < Form<T>::kInner; ++inner) {
+                Fragment<T> fq[W::kC];
+#pragma unroll
+                for (int c = 0; c < W::kC; ++c) fq[c] = rq.get(c, inner);
+#pragma unroll
+                for (int r = 0; r < W::kR; ++r) {
+                    const Fragment<T> fp = rp.get(r, inner);
+#pragma unroll
+                    for (int c = 0; c < W::kC; ++c) acc[r][c] = mma(fq[c], fp, acc[r][c]);
+                    if constexpr (decltype(sums)::value) {
+                        if (r / W::kSums == wave % W::kWaveCols) {
+                            rows_sum[r % W::kSums] = sum_rows(fp, rows_sum[r % W::kSums]);
+                        }
+                    }
+                }
+            }
+        };
+        // two steps a turn; a second one past the end is of zeros (a way out between the two
+        // costs a second set of accumulators)
+        if (length > 0) issue(half0, 0);
+        for (int k = 0; k < length; k += 2 * kStep) {
+            arrive();
+            issue(half1, k + kStep);
+            multiply(p0, q0);
+            arrive();
+            if (k + 2 * kStep < length) issue(half0, k + 2 * kStep);
+            multiply(p1, q1);
+        }
+    };
+    if constexpr (KIND == kLinearGradWeight) {
+        if (w.sums) run(std::true_type{});
+        else run(std::false_type{});
+    } else {
+        run(std::false_type{});
+    }
+    if constexpr (KIND == kLinearGradWeight) {
+        leave_part<kLarge, kLarge>(a, acc, rows_sum, w.part, row0, col0, w.sums);
+    } else {
+        finish<T, TO, kLarge, kLarge, KIND>(a, half0, acc, row0, col0);
     }
 }
 
@@ -735,7 +1091,7 @@ template <typename T, typename TO>
 __global__ __launch_bounds__(kFewThreads) void few_rows_kernel(const Product a) {
     constexpr int kEach = Form<T>::kLane * 4;   // values of k a step
     __shared__ float sums[kFewWaves][16][20];
-    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, g = lane >> 4;
+    const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), g = lane >> 4;
     const int64_t col0 = static_cast<int64_t>(blockIdx.x) * 16, row0 = static_cast<int64_t>(blockIdx.y) * 16;
     const int64_t row = row0 + (lane & 15), col = col0 + (lane & 15);
     const bool has_row = row < a.p.rows, has_col = col < a.q.rows;
@@ -769,19 +1125,22 @@ __global__ __launch_bounds__(kFewThreads) void few_rows_kernel(const Product a) 
     if (j.residual != nullptr) y[0] += as_float(static_cast<const TO*>(j.residual)[out_row * j.residual_stride + out_col]);
     const int64_t o = out_row * a.q.rows + out_col;
     static_cast<TO*>(j.out)[o] = static_cast<TO>(y[0]);
-    if (j.slope_out != nullptr) static_cast<TO*>(j.slope_out)[o] = static_cast<TO>(d[0]);
+    if (j.slope_out != nullptr) {
+        using Slope = typename Form<TO>::Slope;
+        static_cast<Slope*>(j.slope_out)[o] = static_cast<Slope>(d[0]);
+    }
 }
 
 // Joins the parts of a weight's gradient, in their order.
-constexpr int kJoin = 32;   // values a workgroup, eight threads each
+constexpr int kJoinThreads = 256, kJoin = 32;   // values a workgroup, eight threads each
 template <typename T>
-__global__ __launch_bounds__(kThreads) void join_kernel(const float* parts, int64_t values, int64_t bias_values,
+__global__ __launch_bounds__(kJoinThreads) void join_kernel(const float* parts, int64_t values, int64_t bias_values,
                                                         int64_t n_parts, int64_t bias_first, int64_t bias_parts,
                                                         T* weight, T* bias) {
-    __shared__ float sums[kThreads / kJoin][kJoin];
+    __shared__ float sums[kJoinThreads / kJoin][kJoin];
     const int64_t at = static_cast<int64_t>(blockIdx.x) * kJoin + threadIdx.x % kJoin;
     const int group = threadIdx.x / kJoin;
-    constexpr int kGroups = kThreads / kJoin;
+    constexpr int kGroups = kJoinThreads / kJoin;
     const int64_t stride = values + bias_values;
     const bool of_bias = at >= values;
     const int64_t first = of_bias ? bias_first : 0, n = of_bias ? bias_parts : n_parts;
@@ -816,7 +1175,26 @@ int launch(Product a, hipStream_t s) {
     const int64_t tiles = a.row_tiles * a.col_tiles * (KIND == kLinearGradWeight ? a.parts * a.pairs : 1);
     const int64_t groups = (tiles + kXcds - 1) / kXcds * kXcds;
     if (groups > 0x7FFFFFFFll) ASH_FAIL("linear: too many rows");
-    product_kernel<T, TO, BR, BC, KIND><<<static_cast<unsigned>(groups), kThreads, 0, s>>>(a);
+    product_kernel<T, TO, BR, BC, KIND><<<static_cast<unsigned>(groups), Tile<BR, BC>::kThreads, 0, s>>>(a);
+    ASH_LAUNCH_CHECK();
+    return 0;
+}
+
+// Whether the large tiles take an operand: 16-byte pieces, rows that do not overlap, tiles
+// of less than 2^31 bytes.  `across`: values along the rows in memory.
+template <typename T> bool takes_large(const Side& a, int64_t across) {
+    return a.mul == nullptr && reinterpret_cast<uintptr_t>(a.p) % 16 == 0 && a.stride * sizeof(T) % 16 == 0 &&
+           across * sizeof(T) % 16 == 0 && a.stride >= across && a.stride < (1 << 21);
+}
+
+template <typename T, typename TO, int KIND>
+int launch_large(Product a, hipStream_t s) {
+    a.row_tiles = tiles_of(a.p.rows, kLarge);
+    a.col_tiles = tiles_of(a.q.rows, kLarge);
+    const int64_t tiles = a.row_tiles * a.col_tiles * (KIND == kLinearGradWeight ? a.parts * a.pairs : 1);
+    const int64_t groups = (tiles + kXcds - 1) / kXcds * kXcds;
+    if (groups > 0x7FFFFFFFll) ASH_FAIL("linear: too many rows");
+    large_kernel<T, TO, KIND><<<static_cast<unsigned>(groups), kLargeThreads, 0, s>>>(a);
     ASH_LAUNCH_CHECK();
     return 0;
 }
@@ -832,16 +1210,29 @@ int launch_by_size(const Product& a, hipStream_t s) {
             return 0;
         }
     }
-    if (a.q.rows <= 32) return launch<T, TO, 128, 32, KIND>(a, s);
-    if constexpr (KIND == kLinearGradWeight) {   // the parts fill the chip whatever the tile
-        if (a.p.rows <= 64) return launch<T, TO, 64, 64, KIND>(a, s);
+    if constexpr (KIND == kLinearGradWeight) {
+        const WeightTile t = weight_tile(a.q.rows, a.p.rows, ASH_LINEAR_DTYPE);
+        if (t.cols == 32) return launch<T, TO, 128, 32, KIND>(a, s);
+        if (t.rows == 64) return launch<T, TO, 64, 64, KIND>(a, s);
         if constexpr (Form<T>::kParts == 1) {
-            if (a.q.rows > 64) return launch<T, TO, 128, 128, KIND>(a, s);
+            if (t.rows == kLarge && takes_large<T>(a.p, a.p.rows) && takes_large<T>(a.q, a.q.rows) &&
+                (a.pairs == 1 || (takes_large<T>(a.p2, a.p.rows) && takes_large<T>(a.q2, a.q.rows)))) {
+                return launch_large<T, TO, KIND>(a, s);
+            }
+            if (t.rows == kLarge) return launch<T, TO, 128, 128, KIND>(a, s);
+            if (t.cols == 128) return launch<T, TO, 128, 128, KIND>(a, s);
         }
         return launch<T, TO, 128, 64, KIND>(a, s);
     }
+    if (a.q.rows <= 32) return launch<T, TO, 128, 32, KIND>(a, s);
     if (tiles_of(a.p.rows, 128) * tiles_of(a.q.rows, 64) < 256) return launch<T, TO, 64, 64, KIND>(a, s);
     if constexpr (Form<T>::kParts == 1) {
+        if constexpr (KIND != kLinearSecond && !std::is_same<T, WideE4M3>::value) {
+            if (a.q.rows > 128 && tiles_of(a.p.rows, kLarge) * tiles_of(a.q.rows, kLarge) >= 256 &&
+                takes_large<T>(a.p, a.k) && takes_large<T>(a.q, KIND == kLinearForward ? a.k : a.q.rows)) {
+                return launch_large<T, TO, KIND>(a, s);
+            }
+        }
         if (a.q.rows > 64) return launch<T, TO, 128, 128, KIND>(a, s);
     }
     return launch<T, TO, 128, 64, KIND>(a, s);
@@ -858,8 +1249,8 @@ int linear_run<ASH_LINEAR_DTYPE>(LinearKind kind, const LinearJob& j, hipStream_
     a.job = j;
     switch (kind) {
         case kLinearForward:
-            a.p = {j.input, nullptr, j.input_stride, j.rows};
-            a.q = {j.weight, nullptr, j.in, j.cols};
+            a.p = {j.input, nullptr, j.input_stride, j.rows, 1.0f};
+            a.q = {j.weight, nullptr, j.in, j.cols, 1.0f};
             a.k = j.in;
             if constexpr (sizeof(T) == 1) {
                 if (j.out_dtype == ASH_F32) return launch_by_size<WideE4M3, float, kLinearForward>(a, s);
@@ -874,22 +1265,22 @@ int linear_run<ASH_LINEAR_DTYPE>(LinearKind kind, const LinearJob& j, hipStream_
     if constexpr (sizeof(T) > 1) {
         switch (kind) {
             case kLinearSecond:
-                a.p = {j.input, nullptr, j.input_stride, j.rows};
-                a.q = {j.weight, nullptr, j.in, j.cols};
+                a.p = {j.input, nullptr, j.input_stride, j.rows, 1.0f};
+                a.q = {j.weight, nullptr, j.in, j.cols, 1.0f};
                 a.k = j.in;
                 a.other = j.second_input;
                 a.other_stride = j.second_stride;
                 return launch_by_size<T, T, kLinearSecond>(a, s);
             case kLinearGradInput:
-                a.p = {j.grad, j.slope, j.cols, j.rows};
-                a.q = {j.weight, nullptr, j.in, j.in};
+                a.p = {j.grad, j.slope, j.cols, j.rows, j.slope_factor};
+                a.q = {j.weight, nullptr, j.in, j.in, 1.0f};
                 a.k = j.cols;
                 return launch_by_size<T, T, kLinearGradInput>(a, s);
             case kLinearGradWeight: {
-                a.p = {j.grad, j.slope, j.cols, j.cols};
-                a.q = {j.input, nullptr, j.input_stride, j.in};
-                a.p2 = {j.second_grad, j.second_slope, j.cols, j.cols};
-                a.q2 = {j.second_factor, nullptr, j.second_stride, j.in};
+                a.p = {j.grad, j.slope, j.cols, j.cols, j.slope_factor};
+                a.q = {j.input, nullptr, j.input_stride, j.in, 1.0f};
+                a.p2 = {j.second_grad, j.second_slope, j.cols, j.cols, j.slope_factor};
+                a.q2 = {j.second_factor, nullptr, j.second_stride, j.in, 1.0f};
                 a.k = j.rows;
                 a.pairs = j.second_grad != nullptr ? 2 : 1;
                 a.parts = j.splits;
@@ -899,7 +1290,7 @@ int linear_run<ASH_LINEAR_DTYPE>(LinearKind kind, const LinearJob& j, hipStream_
                 if (j.rows > 0 && launch_by_size<T, T, kLinearGradWeight>(a, s) != 0) return 1;
                 const int64_t values = j.cols * j.in, parts = j.rows > 0 ? a.parts * a.pairs : 0;
                 const int64_t groups = tiles_of(values + j.cols, kJoin);
-                join_kernel<T><<<static_cast<unsigned>(groups), kThreads, 0, s>>>(
+                join_kernel<T><<<static_cast<unsigned>(groups), kJoinThreads, 0, s>>>(
                         static_cast<const float*>(j.scratch), values, j.cols, parts,
                         a.second_has_bias ? a.parts : 0, j.rows > 0 ? a.parts : 0, static_cast<T*>(j.out),
                         static_cast<T*>(j.bias_out));
