@@ -81,12 +81,16 @@ __device__ inline int place(int row, int c) {
     }
 }
 
-// The same for rows of k of ROWS values of two bytes, such that the sixteen lanes that are
-// served together by a turning read (four rows of k, 32 bytes of each) meet different banks.
+// The same for rows of k of ROWS values of two bytes, such that the 32 lanes that are served
+// together by a turning read (rows k to k + 3 and k + 8 to k + 11, 32 bytes of each) meet
+// different banks of the 64.
 template <int ROWS>
 __device__ inline int stacked_place(int k, int c) {
-    if constexpr (ROWS >= 64) return k * ROWS * 2 + ((c ^ ((k & 3) << 1)) << 4);
-    else return k * ROWS * 2 + ((c ^ (k & 2)) << 4);
+    int f;
+    if constexpr (ROWS >= 128) f = ((k & 3) << 1) | (k & 8);
+    else if constexpr (ROWS == 64) f = (k & 2) | ((k & 8) >> 1);
+    else f = (k & 8) >> 2;
+    return k * ROWS * 2 + ((c ^ f) << 4);
 }
 
 template <typename T> __device__ inline float as_float(T v) { return static_cast<float>(v); }
@@ -443,7 +447,67 @@ __device__ inline f32x4 sum_rows(const Fragment<float>& p, f32x4 c) {
 }
 
 // --------------------------------------------------------------------- activations
-__device__ inline float sigmoid(float v) { return 1.0f / (1.0f + expf(-v)); }
+// exp(x) by the unit's exp2: the argument's product with log2(e) in two parts, of which the
+// second, below a step of the first, is applied as a factor.
+__device__ inline float exp_of(float x) {
+    const float t = x * 1.44269504f;
+    const float rest = fmaf(x, 1.44269504f, -t) + x * 1.92596299e-8f;
+    const float e = __builtin_amdgcn_exp2f(t);
+    // (beyond the range of float the first part says all there is)
+    return fabsf(rest) < 1.0f ? fmaf(e, rest * 0.69314718f, e) : e;
+}
+
+__device__ inline float sigmoid(float v) { return __builtin_amdgcn_rcpf(1.0f + exp_of(-v)); }
+
+// The normal distribution's integral and its density at z.  The complementary error function
+// is t exp(-x^2 + P(t)), t = 1 / (1 + x / 2), with the Chebyshev fit erfcc of Press et al.,
+// Numerical Recipes (1.2e-7 of the value, everywhere).
+__device__ inline void normal(float z, float& integral, float& density) {
+    const float x = fabsf(z) * 0.70710678f, t = __builtin_amdgcn_rcpf(fmaf(0.5f, x, 1.0f));
+    float p = 0.17087277f;
+    p = fmaf(p, t, -0.82215223f);
+    p = fmaf(p, t, 1.48851587f);
+    p = fmaf(p, t, -1.13520398f);
+    p = fmaf(p, t, 0.27886807f);
+    p = fmaf(p, t, -0.18628806f);
+    p = fmaf(p, t, 0.09678418f);
+    p = fmaf(p, t, 0.37409196f);
+    p = fmaf(p, t, 1.00002368f);
+    p = fmaf(p, t, -1.26551223f);
+    const float e = exp_of(-0.5f * z * z), tail = 0.5f * t * e * exp_of(p);
+    integral = z > 0.0f ? 1.0f - tail : tail;
+    density = 0.39894228f * e;
+}
+
+// log(1 + e), e in [0, 1]
+__device__ inline float log_of_one_and(float e) {
+    const float u = 1.0f + e;
+    const float far = fmaf(__builtin_amdgcn_logf(u), 0.69314718f, (e - (u - 1.0f)) * __builtin_amdgcn_rcpf(u));
+    const float near = e * fmaf(e, fmaf(e, fmaf(e, fmaf(e, 0.2f, -0.25f), 0.33333333f), -0.5f), 1.0f);
+    return e < 0.0625f ? near : far;
+}
+
+// Sine and cosine: the argument less multiples of pi / 2, by a constant in three parts (up
+// to 2^17; in 64 bits beyond, good to 2^40), and the series up to r^9 and r^8.
+__device__ inline void sine_cosine(float x, float& sine, float& cosine) {
+    float k = rintf(x * 0.63661977f);
+    float r = fmaf(k, -1.57079637f, x);
+    r = fmaf(k, 4.37113900e-8f, r);
+    r = fmaf(k, 1.71512489e-15f, r);
+    int quarter = static_cast<int>(k);
+    if (fabsf(x) > 131072.0f) {
+        const double whole = rint(static_cast<double>(x) * 0.63661977236758134);
+        r = static_cast<float>(fma(whole, -6.123233995736766e-17, fma(whole, -1.5707963267948966, static_cast<double>(x))));
+        quarter = static_cast<int>(static_cast<int64_t>(whole));
+    }
+    const float q = r * r;
+    const float s = fmaf(r * q, fmaf(q, fmaf(q, fmaf(q, 2.75573192e-6f, -1.98412698e-4f), 8.33333333e-3f), -0.16666667f), r);
+    const float c = fmaf(q, fmaf(q, fmaf(q, fmaf(q, 2.48015873e-5f, -1.38888889e-3f), 4.16666667e-2f), -0.5f), 1.0f);
+    sine = quarter & 1 ? c : s;
+    cosine = quarter & 1 ? s : c;
+    if (quarter & 2) sine = -sine;
+    if ((quarter + 1) & 2) cosine = -cosine;
+}
 
 // Slopes that are kept for a backward pass are float32, for bf16 operands fp16: a rounding
 // of them to the operands' type would be one more of the size of that of gz and of the
@@ -455,8 +519,7 @@ __device__ inline void activate(int kind, float a, const float (&z)[N], float (&
         case ASH_ACT_RELU:
 #pragma unroll
             for (int i = 0; i < N; ++i) {
-                // NaN stays NaN
-                y[i] = z[i] < 0.0f ? 0.0f : z[i];
+                y[i] = z[i] < 0.0f ? 0.0f : z[i];   // NaN stays NaN
                 d[i] = z[i] > 0.0f ? 1.0f : 0.0f;
             }
             break;
@@ -465,34 +528,31 @@ __device__ inline void activate(int kind, float a, const float (&z)[N], float (&
             for (int i = 0; i < N; ++i) {
                 const float p = sigmoid(z[i]);
                 y[i] = z[i] * p;
-                d[i] = p * (1.0f + z[i] * (1.0f - p));
+                d[i] = p * fmaf(z[i], 1.0f - p, 1.0f);
             }
             break;
         case ASH_ACT_GELU:
 #pragma unroll
             for (int i = 0; i < N; ++i) {
-                const float c = 0.5f * erfcf(-0.70710678f * z[i]);
+                float c, density;
+                normal(z[i], c, density);
                 y[i] = z[i] * c;
-                d[i] = c + z[i] * 0.39894228f * expf(-0.5f * z[i] * z[i]);
+                d[i] = fmaf(z[i], density, c);
             }
             break;
-        case ASH_ACT_SOFTPLUS:
+        case ASH_ACT_SOFTPLUS: {
+            const float inverse = 1.0f / a;
 #pragma unroll
             for (int i = 0; i < N; ++i) {
-                const float v = a * z[i], e = expf(-fabsf(v));
-                y[i] = (v > 0.0f ? z[i] : 0.0f) + log1pf(e) / a;
-                d[i] = (v > 0.0f ? 1.0f : e) / (1.0f + e);
-                if (v != v) y[i] = d[i] = v;
+                const float v = a * z[i], e = exp_of(-fabsf(v)), r = __builtin_amdgcn_rcpf(1.0f + e);
+                y[i] = fmaf(log_of_one_and(e), inverse, v < 0.0f ? 0.0f : z[i]);
+                d[i] = v < 0.0f ? e * r : r;
             }
             break;
+        }
         case ASH_ACT_SINE:
 #pragma unroll
-            for (int i = 0; i < N; ++i) {
-                float s, c;
-                sincosf(a * z[i], &s, &c);
-                y[i] = s;
-                d[i] = c;
-            }
+            for (int i = 0; i < N; ++i) sine_cosine(a * z[i], y[i], d[i]);
             break;
         default:
 #pragma unroll
@@ -503,6 +563,7 @@ __device__ inline void activate(int kind, float a, const float (&z)[N], float (&
     }
 }
 
+// f'(z) (whole, of a sine too) and f''(z)
 template <int N>
 __device__ inline void curve(int kind, float a, const float (&z)[N], float (&d)[N], float (&dd)[N]) {
     switch (kind) {
@@ -510,23 +571,24 @@ __device__ inline void curve(int kind, float a, const float (&z)[N], float (&d)[
 #pragma unroll
             for (int i = 0; i < N; ++i) {
                 const float p = sigmoid(z[i]);
-                d[i] = p * (1.0f + z[i] * (1.0f - p));
-                dd[i] = p * (1.0f - p) * (2.0f + z[i] * (1.0f - 2.0f * p));
+                d[i] = p * fmaf(z[i], 1.0f - p, 1.0f);
+                dd[i] = p * (1.0f - p) * fmaf(z[i], 1.0f - 2.0f * p, 2.0f);
             }
             break;
         case ASH_ACT_GELU:
 #pragma unroll
             for (int i = 0; i < N; ++i) {
-                const float density = 0.39894228f * expf(-0.5f * z[i] * z[i]);
-                d[i] = 0.5f * erfcf(-0.70710678f * z[i]) + z[i] * density;
-                dd[i] = (2.0f - z[i] * z[i]) * density;
+                float c, density;
+                normal(z[i], c, density);
+                d[i] = fmaf(z[i], density, c);
+                dd[i] = fmaf(-z[i], z[i], 2.0f) * density;
             }
             break;
         case ASH_ACT_SOFTPLUS:
 #pragma unroll
             for (int i = 0; i < N; ++i) {
-                const float v = a * z[i], e = expf(-fabsf(v)), r = 1.0f / (1.0f + e);
-                d[i] = v > 0.0f ? r : e * r;
+                const float v = a * z[i], e = exp_of(-fabsf(v)), r = __builtin_amdgcn_rcpf(1.0f + e);
+                d[i] = v < 0.0f ? e * r : r;
                 dd[i] = a * e * r * r;
             }
             break;
@@ -534,7 +596,7 @@ __device__ inline void curve(int kind, float a, const float (&z)[N], float (&d)[
 #pragma unroll
             for (int i = 0; i < N; ++i) {
                 float s, c;
-                sincosf(a * z[i], &s, &c);
+                sine_cosine(a * z[i], s, c);
                 d[i] = a * c;
                 dd[i] = -a * a * s;
             }
@@ -618,7 +680,7 @@ struct Tile {
     static constexpr int kWaveRows = kWaves / kWaveCols;
     static constexpr int kR = BR / kWaveRows / 16, kC = BC / kWaveCols / 16;
     static constexpr int kSums = kR / kWaveCols;   // rows of P are summed by those that share them, so many of kR each
-    static constexpr int kPass = kR > 4 ? 2 : kR, kPasses = kR / kPass;   // of kR
+    static constexpr int kPass = kR > 4 ? 1 : kR, kPasses = kR / kPass;   // of kR
     static constexpr int kOutRows = kWaveRows * kPass * 16;
 };
 
@@ -631,11 +693,12 @@ template <typename T, int BR, int BC> struct Shared {
     static constexpr int kBytes = 2 * (kP + kQ) > kOut ? 2 * (kP + kQ) : kOut;
 };
 
-// The way out of a tile's sums.  They go through LDS once more, so that a thread has eight
-// columns of a row: operands and results then come and go in whole lines.
-template <typename T, typename TO, int BR, int BC, int KIND, int PASS>
-__device__ inline void finish_pass(const Product& a, char* lds, const f32x4 (&acc)[Tile<BR, BC>::kR][Tile<BR, BC>::kC],
-                                   int64_t row0, int64_t col0, const float (&bias)[8], const float (&scale)[8]) {
+// The way out of a tile's sums.  They go through LDS once more, some rows of every wavefront
+// at a time, so that a thread has eight columns of a row: operands and results then come and
+// go in whole lines.
+template <typename T, typename TO, int BR, int BC, int KIND>
+__device__ inline void finish(const Product& a, char* lds, const f32x4 (&acc)[Tile<BR, BC>::kR][Tile<BR, BC>::kC],
+                              int64_t row0, int64_t col0) {
     using W = Tile<BR, BC>;
     constexpr int kStride = Shared<T, BR, BC>::kStride;
     constexpr int kAcross = BC / 8, kDown = W::kThreads / kAcross;
@@ -643,83 +706,83 @@ __device__ inline void finish_pass(const Product& a, char* lds, const f32x4 (&ac
     const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
     const int wave_col = wave % W::kWaveCols * W::kC * 16;
     float* sums_of = reinterpret_cast<float*>(lds);
-    __syncthreads();
-#pragma unroll
-    for (int r = 0; r < W::kPass; ++r) {
-#pragma unroll
-        for (int c = 0; c < W::kC; ++c) {
-            *reinterpret_cast<f32x4*>(sums_of + ((wave / W::kWaveCols * W::kPass + r) * 16 + (lane & 15)) * kStride +
-                                      wave_col + c * 16 + (lane >> 4) * 4) = acc[PASS * W::kPass + r][c];
-        }
-    }
-    __syncthreads();
     const LinearJob& j = a.job;
     const int at = threadIdx.x % kAcross * 8;
     const int64_t col = col0 + at, left = a.q.rows - col;
-#pragma unroll 1
-    for (int r = threadIdx.x / kAcross; r < kPassRows; r += kDown) {
-        // rows 16 kPass w and on of a pass are those of the wavefronts' row w
-        const int64_t row = row0 + r / (W::kPass * 16) * W::kR * 16 + PASS * W::kPass * 16 + r % (W::kPass * 16);
-        if (row >= a.p.rows || left <= 0) continue;
-        float z[8], y[8], d[8];
-        const float row_scale = Form<T>::kScaled ? j.input_scales[row] : 1.0f;
-#pragma unroll
-        for (int i = 0; i < 8; ++i) {
-            z[i] = sums_of[r * kStride + at + i];
-            if constexpr (Form<T>::kScaled) z[i] *= row_scale * scale[i];
-            z[i] += bias[i];
-        }
-        const int64_t o = row * a.q.rows + col;
-        if constexpr (KIND == kLinearSecond) {
-            // t: the derivative of <second input, gradient of the input> by gz
-            float t[8], g[8], dd[8];
-#pragma unroll
-            for (int i = 0; i < 8; ++i) t[i] = sums_of[(kPassRows + r) * kStride + at + i];
-            if (j.addend != nullptr) {
-                float more[8];
-                read8(static_cast<const TO*>(j.addend) + row * j.addend_stride + col, left, more);
-#pragma unroll
-                for (int i = 0; i < 8; ++i) t[i] += more[i];
-            }
-            read8(static_cast<const TO*>(j.grad) + o, left, g);
-            curve(j.activation, j.act_scale, z, d, dd);
-#pragma unroll
-            for (int i = 0; i < 8; ++i) {
-                y[i] = t[i] * d[i];
-                dd[i] *= t[i] * g[i];
-            }
-            if (j.out != nullptr) write8(static_cast<TO*>(j.out) + o, left, y);
-            if (j.curvature_out != nullptr) write8(static_cast<TO*>(j.curvature_out) + o, left, dd);
-        } else {
-            activate(j.activation, j.act_scale, z, y, d);
-            if (j.residual != nullptr) {
-                float more[8];
-                read8(static_cast<const TO*>(j.residual) + row * j.residual_stride + col, left, more);
-#pragma unroll
-                for (int i = 0; i < 8; ++i) y[i] += more[i];
-            }
-            write8(static_cast<TO*>(j.out) + o, left, y);
-            if (j.slope_out != nullptr) write8(static_cast<typename Form<TO>::Slope*>(j.slope_out) + o, left, d);
-        }
-    }
-    if constexpr (PASS + 1 < W::kPasses) {
-        finish_pass<T, TO, BR, BC, KIND, PASS + 1>(a, lds, acc, row0, col0, bias, scale);
-    }
-}
-
-template <typename T, typename TO, int BR, int BC, int KIND>
-__device__ inline void finish(const Product& a, char* lds, const f32x4 (&acc)[Tile<BR, BC>::kR][Tile<BR, BC>::kC],
-                              int64_t row0, int64_t col0) {
-    const int64_t col = col0 + threadIdx.x % (BC / 8) * 8, left = a.q.rows - col;
     float bias[8], scale[8];
 #pragma unroll
     for (int i = 0; i < 8; ++i) {
         bias[i] = 0.0f;
         scale[i] = 1.0f;
     }
-    if (a.job.bias != nullptr) read8(static_cast<const TO*>(a.job.bias) + col, left, bias);
-    if constexpr (Form<T>::kScaled) read8(a.job.weight_scales + col, left, scale);
-    finish_pass<T, TO, BR, BC, KIND, 0>(a, lds, acc, row0, col0, bias, scale);
+    if (j.bias != nullptr) read8(static_cast<const TO*>(j.bias) + col, left, bias);
+    if constexpr (Form<T>::kScaled) read8(j.weight_scales + col, left, scale);
+#pragma unroll 1
+    for (int pass = 0; pass < W::kPasses; ++pass) {
+        __syncthreads();
+        // (accumulators are registers: which of them is said in the code, and the rest of it is
+        // there once)
+#pragma unroll
+        for (int now = 0; now < W::kPasses; ++now) {
+            if (now != pass) continue;
+#pragma unroll
+            for (int r = 0; r < W::kPass; ++r) {
+#pragma unroll
+                for (int c = 0; c < W::kC; ++c) {
+                    *reinterpret_cast<f32x4*>(sums_of +
+                                              ((wave / W::kWaveCols * W::kPass + r) * 16 + (lane & 15)) * kStride +
+                                              wave_col + c * 16 + (lane >> 4) * 4) = acc[now * W::kPass + r][c];
+                }
+            }
+        }
+        __syncthreads();
+#pragma unroll 1
+        for (int r = threadIdx.x / kAcross; r < kPassRows; r += kDown) {
+            // rows 16 kPass w and on of a pass are those of the wavefronts' row w
+            const int64_t row = row0 + r / (W::kPass * 16) * W::kR * 16 + pass * W::kPass * 16 + r % (W::kPass * 16);
+            if (row >= a.p.rows || left <= 0) continue;
+            float z[8], y[8], d[8];
+            const float row_scale = Form<T>::kScaled ? j.input_scales[row] : 1.0f;
+#pragma unroll
+            for (int i = 0; i < 8; ++i) {
+                z[i] = sums_of[r * kStride + at + i];
+                if constexpr (Form<T>::kScaled) z[i] *= row_scale * scale[i];
+                z[i] += bias[i];
+            }
+            const int64_t o = row * a.q.rows + col;
+            if constexpr (KIND == kLinearSecond) {
+                // t: the derivative of <second input, gradient of the input> by gz
+                float t[8], g[8], dd[8];
+#pragma unroll
+                for (int i = 0; i < 8; ++i) t[i] = sums_of[(kPassRows + r) * kStride + at + i];
+                if (j.addend != nullptr) {
+                    float more[8];
+                    read8(static_cast<const TO*>(j.addend) + row * j.addend_stride + col, left, more);
+#pragma unroll
+                    for (int i = 0; i < 8; ++i) t[i] += more[i];
+                }
+                read8(static_cast<const TO*>(j.grad) + o, left, g);
+                curve(j.activation, j.act_scale, z, d, dd);
+#pragma unroll
+                for (int i = 0; i < 8; ++i) {
+                    y[i] = t[i] * d[i];
+                    dd[i] *= t[i] * g[i];
+                }
+                if (j.out != nullptr) write8(static_cast<TO*>(j.out) + o, left, y);
+                if (j.curvature_out != nullptr) write8(static_cast<TO*>(j.curvature_out) + o, left, dd);
+            } else {
+                activate(j.activation, j.act_scale, z, y, d);
+                if (j.residual != nullptr) {
+                    float more[8];
+                    read8(static_cast<const TO*>(j.residual) + row * j.residual_stride + col, left, more);
+#pragma unroll
+                    for (int i = 0; i < 8; ++i) y[i] += more[i];
+                }
+                write8(static_cast<TO*>(j.out) + o, left, y);
+                if (j.slope_out != nullptr) write8(static_cast<typename Form<TO>::Slope*>(j.slope_out) + o, left, d);
+            }
+        }
+    }
 }
 
 // A part's sums of a weight's gradient, in float32; join_kernel joins the parts.
@@ -874,17 +937,37 @@ __global__ __launch_bounds__((Tile<BR, BC>::kThreads)) void product_kernel(const
 
 // Large products of operands of one or two bytes: tiles of 256 x 256, whose operands go from
 // memory into LDS without passing through registers, so that a wavefront can hold 128 x 64
-// sums (with 64 x 64 a wavefront the reads from LDS take as long as the products).  Both
-// halves of a step's 16-byte pieces are addressed such that they land where place() and
-// stacked_place() look for them.  Pieces past an operand's end, and past the last k, are
-// outside of the buffer that the loads are told of, and come as zeros.
-constexpr int kLarge = 256, kLargeThreads = 512, kLargeEach = 4;   // pieces a thread, operand and step
-constexpr uint32_t kNowhere = 0x80000000u;                         // beyond every such buffer
+// sums (with 64 x 64 a wavefront the reads from LDS take as long as the products).  The
+// 16-byte pieces of a stage are fetched such that they land where Reader looks for them.
+// Pieces past an operand's end, and past the last k, are outside of the buffer that the
+// loads are told of, and come as zeros.
+//
+// bf16, fp16: four stages of 32 values of k, of which three are on their way while one is
+// multiplied; e4m3, whose instructions take 128 values of k, two.
+constexpr int kLarge = 256, kLargeThreads = 512;
+constexpr uint32_t kNowhere = 0x80000000u;   // beyond every such buffer
+
+template <typename T> struct Stage {
+    static constexpr int kRow = Form<T>::kIsByte ? 128 : 64;        // bytes of k
+    static constexpr int kK = kRow / static_cast<int>(sizeof(T));   // values of k
+    static constexpr int kStages = Form<T>::kIsByte ? 2 : 4;
+    static constexpr int kEach = kLarge * kRow / 16 / kLargeThreads;   // pieces a thread and operand
+    static constexpr int kPlane = kLarge * kRow;
+    // stacked: 128 bytes more for every eight rows of k, which puts the rows that a turning
+    // read takes together on different banks
+    static constexpr int kStacked = kPlane + kK / 8 * 128;
+    // until all but the newest stages have come, and all reads from LDS (s_waitcnt: vmcnt in
+    // bits 0-3 and 14-15, lgkmcnt in 8-11)
+    static constexpr int kUnderWay = (kStages - 2) * 2 * kEach;
+    static constexpr int kWait = 0x0070 | (kUnderWay & 15) | (kUnderWay >> 4 << 14);
+};
+constexpr int kWaitAll = 0x0070;
 
 template <typename T, bool STACKED>
 struct Direct {
+    using S = Stage<T>;
     const char* base;       // of the tile, at the first k
-    uint32_t offset[kLargeEach], stride;
+    uint32_t offset[S::kEach], stride;
     int k_of;               // first k of this thread's pieces along a row
     int64_t extent;         // bytes from base to the operand's end (of k_end)
 
@@ -900,14 +983,15 @@ struct Direct {
         }
         k_of = 0;
 #pragma unroll
-        for (int i = 0; i < kLargeEach; ++i) {
+        for (int i = 0; i < S::kEach; ++i) {
             const int piece = threadIdx.x + i * kLargeThreads;
             if constexpr (STACKED) {
                 const int k = piece >> 5, c = (piece & 31) ^ ((k & 3) << 1);
                 offset[i] = k * stride + c * 16;
             } else {
-                const int row = piece >> 3, c = (piece & 7) ^ (row & 7);
-                k_of = c * Form<T>::kChunk;
+                constexpr int kPieces = S::kRow / 16;
+                const int row = piece / kPieces, c = (piece ^ (kPieces == 8 ? row & 7 : (row >> 2) & 3)) % kPieces;
+                k_of = c * Form<T>::kChunk;   // (the same for every i)
                 offset[i] = row * stride + c * 16;
             }
         }
@@ -919,148 +1003,209 @@ struct Direct {
         const auto buffer = __builtin_amdgcn_make_buffer_rsrc(
                 const_cast<char*>(base + past), 0, static_cast<int>(left < 0x7FFFFFFF ? left : 0x7FFFFFFF), 0x00020000);
         const bool there = STACKED || k_of < k_left;
+        const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
 #pragma unroll
-        for (int i = 0; i < kLargeEach; ++i) {
-            // a wavefront's pieces are consecutive
-            char* at = plane + __builtin_amdgcn_readfirstlane(threadIdx.x >> 6) * 1024 + i * kLargeThreads * 16;
+        for (int i = 0; i < S::kEach; ++i) {
+            // a wavefront's pieces are consecutive: stacked, those of two rows of k
+            char* at = plane + wave * 1024 + i * kLargeThreads * 16;
+            if constexpr (STACKED) at += ((wave >> 2) + i * 2) * 128;
             __builtin_amdgcn_raw_ptr_buffer_load_lds(
                     buffer, (__attribute__((address_space(3))) void*)at, 16, there ? offset[i] : kNowhere, 0, 0, 0);
         }
     }
 };
 
-// Where a lane's pieces lie: addresses differ from one another by constants (Along), or go
-// round in four (Stacked), so that a wavefront keeps a few of them in registers.
+// Where a lane's pieces lie in a stage: addresses differ from one another by constants, or
+// (stacked) go round in four, so that a wavefront keeps a few of them in registers.
 template <typename T, bool STACKED>
 struct Reader {
-    const char* at[STACKED ? 4 : 2];
+    static constexpr int kAt = STACKED ? 4 : Form<T>::kIsByte ? 2 : 1;
+    const char* at[kAt];
 
     __device__ Reader(const char* plane, int row0) {
         const int lane = threadIdx.x & 63, i = lane & 15, g = lane >> 4;
-        if constexpr (STACKED) {
-            const int k = g * 8 + (i >> 2);
 #pragma unroll
-            for (int n = 0; n < 4; ++n) {
-                at[n] = plane + k * kLarge * 2 + ((((row0 >> 3) + ((i & 3) >> 1)) ^ (((k & 3) ^ n) << 1)) << 4) + (i & 1) * 8;
+        for (int n = 0; n < kAt; ++n) {
+            if constexpr (STACKED) {
+                const int k = g * 8 + (i >> 2), c = ((row0 >> 3) + ((i & 3) >> 1)) ^ (((k & 3) ^ n) << 1);
+                at[n] = plane + k * kLarge * 2 + g * 128 + (c << 4) + (i & 1) * 8;
+            } else if constexpr (Form<T>::kIsByte) {
+                at[n] = plane + (row0 + i) * 128 + (((2 * g + n) ^ (i & 7)) << 4);
+            } else {
+                at[n] = plane + (row0 + i) * 64 + ((g ^ (i >> 2)) << 4);
             }
-        } else if constexpr (Form<T>::kIsByte) {
-#pragma unroll
-            for (int n = 0; n < 2; ++n) at[n] = plane + (row0 + i) * 128 + (((2 * g + n) ^ (i & 7)) << 4);
-        } else {
-#pragma unroll
-            for (int n = 0; n < 2; ++n) at[n] = plane + (row0 + i) * 128 + (((4 * n + g) ^ (i & 7)) << 4);
         }
     }
-    // rows 16 r and on from row0
-    __device__ Fragment<T> get(int r, int inner) const {
-        Fragment<T> f;
+    // rows 16 (4 QUAD) and on from row0: four fragments
+    template <int QUAD>
+    __device__ void get(Fragment<T> (&f)[4]) const {
         if constexpr (STACKED) {
-            i16x4 part[2];
+            // The compiler takes a turning read to need whatever is on its way into LDS, and
+            // would wait for the stages to come; so they are written out, with their wait.
+            i16x4 part[8];
+#if defined(__HIP_DEVICE_COMPILE__)
+            uint32_t from[4];
 #pragma unroll
-            for (int h = 0; h < 2; ++h) {
-                const char* p = at[r & 3] + (r >> 2) * 128 + (inner * 32 + h * 4) * kLarge * 2;
-                part[h] = __builtin_amdgcn_ds_read_tr16_b64_v4i16(
-                        (__attribute__((address_space(3))) i16x4*)const_cast<char*>(p));
+            for (int n = 0; n < 4; ++n) {
+                from[n] = static_cast<uint32_t>(reinterpret_cast<uintptr_t>(
+                        (__attribute__((address_space(3))) const char*)at[n]));
             }
-            __builtin_memcpy(&f.v, part, 16);
-        } else if constexpr (Form<T>::kIsByte) {
-            uint4 part[2];
+            asm volatile(
+                    "ds_read_b64_tr_b16 %0, %8 offset:%12\n\t"
+                    "ds_read_b64_tr_b16 %1, %8 offset:%13\n\t"
+                    "ds_read_b64_tr_b16 %2, %9 offset:%12\n\t"
+                    "ds_read_b64_tr_b16 %3, %9 offset:%13\n\t"
+                    "ds_read_b64_tr_b16 %4, %10 offset:%12\n\t"
+                    "ds_read_b64_tr_b16 %5, %10 offset:%13\n\t"
+                    "ds_read_b64_tr_b16 %6, %11 offset:%12\n\t"
+                    "ds_read_b64_tr_b16 %7, %11 offset:%13\n\t"
+                    "s_waitcnt lgkmcnt(0)"
+                    : "=&v"(part[0]), "=&v"(part[1]), "=&v"(part[2]), "=&v"(part[3]), "=&v"(part[4]), "=&v"(part[5]),
+                      "=&v"(part[6]), "=&v"(part[7])
+                    : "v"(from[0]), "v"(from[1]), "v"(from[2]), "v"(from[3]), "n"(QUAD * 128),
+                      "n"(QUAD * 128 + 4 * kLarge * 2)
+                    : "memory");
+#endif
 #pragma unroll
-            for (int n = 0; n < 2; ++n) part[n] = *reinterpret_cast<const uint4*>(at[n] + r * 2048);
-            __builtin_memcpy(&f.v, part, 32);
+            for (int r = 0; r < 4; ++r) __builtin_memcpy(&f[r].v, part + 2 * r, 16);
         } else {
-            __builtin_memcpy(&f.v, at[inner] + r * 2048, 16);
+#pragma unroll
+            for (int r = 0; r < 4; ++r) {
+                if constexpr (Form<T>::kIsByte) {
+                    uint4 part[2];
+#pragma unroll
+                    for (int n = 0; n < 2; ++n) {
+                        part[n] = *reinterpret_cast<const uint4*>(at[n] + (QUAD * 4 + r) * 2048);
+                    }
+                    __builtin_memcpy(&f[r].v, part, 32);
+                } else {
+                    __builtin_memcpy(&f[r].v, at[0] + (QUAD * 4 + r) * 1024, 16);
+                }
+            }
         }
-        return f;
     }
 };
 
-constexpr int kWaitLoads = 0x0F70;   // until no load from memory is under way
+using LargeTile = Tile<kLarge, kLarge>;
+static_assert(LargeTile::kC == 4 && LargeTile::kR == 8 && LargeTile::kThreads == kLargeThreads, "");
+
+template <typename T, int QUAD, bool SUMS>
+__device__ inline void multiply_quad(const Fragment<T> (&fq)[4], const Fragment<T> (&fp)[4],
+                                     f32x4 (&acc)[LargeTile::kR][4], f32x4 (&rows_sum)[LargeTile::kSums], int wave) {
+    using W = LargeTile;
+#pragma unroll
+    for (int n = 0; n < 4; ++n) {
+        const int r = QUAD * 4 + n;
+#pragma unroll
+        for (int c = 0; c < 4; ++c) acc[r][c] = mma(fq[c], fp[n], acc[r][c]);
+        if constexpr (SUMS) {
+            if (r / W::kSums == wave % W::kWaveCols) rows_sum[r % W::kSums] = sum_rows(fp[n], rows_sum[r % W::kSums]);
+        }
+    }
+}
+
+// What a wavefront has of a large tile, and what it does in a step.  SUMS: the sums of P's
+// rows too (by the workgroups that are the first of a row of tiles).
+template <typename T, bool STACK_P, bool STACK_Q>
+struct LargeWork {
+    using W = LargeTile;
+    using S = Stage<T>;
+    static constexpr int kP = STACK_P ? S::kStacked : S::kPlane, kQ = STACK_Q ? S::kStacked : S::kPlane;
+    Direct<T, STACK_P> p;
+    Direct<T, STACK_Q> q;
+    int length, wave;
+    f32x4 acc[W::kR][W::kC], rows_sum[W::kSums];
+
+    __device__ void start(const Side& sp, const Side& sq, int64_t row0, int64_t col0, int64_t k0, int64_t k_end) {
+        p.start(sp, row0, k0, k_end);
+        q.start(sq, col0, k0, k_end);
+        length = k_end > k0 ? static_cast<int>(k_end - k0) : 0;
+        wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+#pragma unroll
+        for (int r = 0; r < W::kSums; ++r) rows_sum[r] = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
+#pragma unroll
+        for (int r = 0; r < W::kR; ++r) {
+#pragma unroll
+            for (int c = 0; c < W::kC; ++c) acc[r][c] = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
+        }
+    }
+    struct Planes {
+        char* p;
+        char* q;
+    };
+    __device__ void issue(const Planes& to, int k) {
+        p.issue(to.p, k, length - k);
+        q.issue(to.q, k, length - k);
+    }
+    template <bool SUMS>
+    __device__ void step(const Planes& stage, const Planes& next, int k_next) {
+        // the stage's operands are there, and nobody reads the next to be filled any more
+        // (__syncthreads would wait for the stages under way too)
+        __builtin_amdgcn_s_waitcnt(S::kWait);
+        asm volatile("" ::: "memory");
+        __builtin_amdgcn_s_barrier();
+        asm volatile("" ::: "memory");
+        issue(next, k_next);
+        const Reader<T, STACK_P> rp(stage.p, wave / W::kWaveCols * W::kR * 16);
+        const Reader<T, STACK_Q> rq(stage.q, wave % W::kWaveCols * W::kC * 16);
+        Fragment<T> fq[4], fp[4];
+        rq.template get<0>(fq);
+        rp.template get<0>(fp);
+        multiply_quad<T, 0, SUMS>(fq, fp, acc, rows_sum, wave);
+        rp.template get<1>(fp);
+        multiply_quad<T, 1, SUMS>(fq, fp, acc, rows_sum, wave);
+    }
+    // All stages a turn; those past the end are of zeros (a way out between them costs a
+    // second set of accumulators).
+    template <bool SUMS>
+    __device__ void run(const Planes& stage0, const Planes& stage1, const Planes& stage2, const Planes& stage3) {
+        constexpr int kK = S::kK;
+        if constexpr (S::kStages == 4) {
+            issue(stage0, 0);
+            issue(stage1, kK);
+            issue(stage2, 2 * kK);
+            for (int k = 0; k < length; k += 4 * kK) {
+                step<SUMS>(stage0, stage3, k + 3 * kK);
+                step<SUMS>(stage1, stage0, k + 4 * kK);
+                step<SUMS>(stage2, stage1, k + 5 * kK);
+                step<SUMS>(stage3, stage2, k + 6 * kK);
+            }
+        } else {
+            issue(stage0, 0);
+            for (int k = 0; k < length; k += 2 * kK) {
+                step<SUMS>(stage0, stage1, k + kK);
+                step<SUMS>(stage1, stage0, k + 2 * kK);
+            }
+        }
+        __builtin_amdgcn_s_waitcnt(kWaitAll);   // nothing may land in LDS from here on
+    }
+};
 
 template <typename T, typename TO, int KIND>
 __global__ __launch_bounds__(kLargeThreads) void large_kernel(const Product a) {
-    using W = Tile<kLarge, kLarge>;
-    constexpr int kPlane = kLarge * 128, kStep = Form<T>::kStep;
     constexpr bool kStackP = KIND == kLinearGradWeight, kStackQ = KIND != kLinearForward;
-    static_assert(W::kThreads == kLargeThreads && W::kOutRows * (kLarge + 4) * 4 <= 2 * 2 * kPlane, "");
-    // two halves under names of their own: reads of one need not wait for loads into the other
-    __shared__ __attribute__((aligned(16))) char half0[2 * kPlane];
-    __shared__ __attribute__((aligned(16))) char half1[2 * kPlane];
+    using Work = LargeWork<T, kStackP, kStackQ>;
+    constexpr int kOut = LargeTile::kOutRows * (kLarge + 4) * 4;
+    constexpr bool kFour = Stage<T>::kStages > 2;
+    // Planes under names of their own: the compiler then sees that reads of one need not wait
+    // for loads into another (it looks only so far through an address, hence one each).
+    __shared__ __attribute__((aligned(16))) char p0[Work::kP > kOut ? Work::kP : kOut];
+    __shared__ __attribute__((aligned(16))) char p1[Work::kP], p2[kFour ? Work::kP : 16], p3[kFour ? Work::kP : 16];
+    __shared__ __attribute__((aligned(16))) char q0[Work::kQ], q1[Work::kQ], q2[kFour ? Work::kQ : 16],
+            q3[kFour ? Work::kQ : 16];
 
     Place w;
     if (!place_of<KIND>(a, w)) return;
     const int64_t row0 = w.row_tile * kLarge, col0 = w.col_tile * kLarge;
-    const int length = w.k_end > w.k0 ? static_cast<int>(w.k_end - w.k0) : 0;
-    Direct<T, kStackP> p;
-    Direct<T, kStackQ> q;
-    p.start(w.second ? a.p2 : a.p, row0, w.k0, w.k_end);
-    q.start(w.second ? a.q2 : a.q, col0, w.k0, w.k_end);
-
-    // (matrix instructions do not go by the mask of lanes: what they depend on has to be known
-    // to be the same for a wavefront)
-    const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
-    const int wave_row = wave / W::kWaveCols * W::kR * 16, wave_col = wave % W::kWaveCols * W::kC * 16;
-    f32x4 acc[W::kR][W::kC], rows_sum[W::kSums];
-#pragma unroll
-    for (int r = 0; r < W::kSums; ++r) rows_sum[r] = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
-#pragma unroll
-    for (int r = 0; r < W::kR; ++r) {
-#pragma unroll
-        for (int c = 0; c < W::kC; ++c) acc[r][c] = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
-    }
-    const auto issue = [&](char* half, int k) {
-        p.issue(half, k, length - k);
-        q.issue(half + kPlane, k, length - k);
-    };
-    const auto arrive = [&] {
-        __builtin_amdgcn_s_waitcnt(kWaitLoads);
-        __syncthreads();   // a step's operands are there, and nobody reads the other half any more
-    };
-    // sums: of P's rows too (by the workgroups that are the first of a row of tiles)
-    const auto run = [&](auto sums) {
-        const Reader<T, kStackP> p0(half0, wave_row), p1(half1, wave_row);
-        const Reader<T, kStackQ> q0(half0 + kPlane, wave_col), q1(half1 + kPlane, wave_col);
-        const auto multiply = [&](const auto& rp, const auto& rq) {
-#pragma unroll
-            for (int inner = 0; inner < Form<T>::kInner; ++inner) {
-                Fragment<T> fq[W::kC];
-#pragma unroll
-                for (int c = 0; c < W::kC; ++c) fq[c] = rq.get(c, inner);
-#pragma unroll
-                for (int r = 0; r < W::kR; ++r) {
-                    const Fragment<T> fp = rp.get(r, inner);
-#pragma unroll
-                    for (int c = 0; c < W::kC; ++c) acc[r][c] = mma(fq[c], fp, acc[r][c]);
-                    if constexpr (decltype(sums)::value) {
-                        if (r / W::kSums == wave % W::kWaveCols) {
-                            rows_sum[r % W::kSums] = sum_rows(fp, rows_sum[r % W::kSums]);
-                        }
-                    }
-                }
-            }
-        };
-        // two steps a turn; a second one past the end is of zeros (a way out between the two
-        // costs a second set of accumulators)
-        if (length > 0) issue(half0, 0);
-        for (int k = 0; k < length; k += 2 * kStep) {
-            arrive();
-            issue(half1, k + kStep);
-            multiply(p0, q0);
-            arrive();
-            if (k + 2 * kStep < length) issue(half0, k + 2 * kStep);
-            multiply(p1, q1);
-        }
-    };
+    Work work;
+    work.start(w.second ? a.p2 : a.p, w.second ? a.q2 : a.q, row0, col0, w.k0, w.k_end);
     if constexpr (KIND == kLinearGradWeight) {
-        if (w.sums) run(std::true_type{});
-        else run(std::false_type{});
+        if (w.sums) work.template run<true>({p0, q0}, {p1, q1}, {p2, q2}, {p3, q3});
+        else work.template run<false>({p0, q0}, {p1, q1}, {p2, q2}, {p3, q3});
+        leave_part<kLarge, kLarge>(a, work.acc, work.rows_sum, w.part, row0, col0, w.sums);
     } else {
-        run(std::false_type{});
-    }
-    if constexpr (KIND == kLinearGradWeight) {
-        leave_part<kLarge, kLarge>(a, acc, rows_sum, w.part, row0, col0, w.sums);
-    } else {
-        finish<T, TO, kLarge, kLarge, KIND>(a, half0, acc, row0, col0);
+        work.template run<false>({p0, q0}, {p1, q1}, {p2, q2}, {p3, q3});
+        finish<T, TO, kLarge, kLarge, KIND>(a, p0, work.acc, row0, col0);
     }
 }
 
