@@ -187,9 +187,9 @@ struct Along {
     Values<T, N> v[kEach];
     Values<M, N> w[kEach];
 
-    // kHalves: rows ROWS / 2 and beyond are rows of another operand of the same shape, zeros
+    // kTwo: every other sixteen rows are rows of another operand of the same shape, zeros
     // where there is none (second order)
-    template <bool kHalves>
+    template <bool kTwo>
     __device__ void start(const Side& a, int64_t row0, const void* other, int64_t other_stride) {
         chunk = threadIdx.x % kChunks;
         mul = MUL && a.mul != nullptr;
@@ -200,10 +200,12 @@ struct Along {
             int r = row[i];
             const T* base = static_cast<const T*>(a.p);
             int64_t stride = a.stride;
-            if (kHalves && r >= ROWS / 2) {
-                r -= ROWS / 2;
-                base = static_cast<const T*>(other);
-                stride = other_stride;
+            if (kTwo) {
+                if (r & 16) {
+                    base = static_cast<const T*>(other);
+                    stride = other_stride;
+                }
+                r = r / 32 * 16 + r % 16;
             }
             const bool there = base != nullptr && row[i] < ROWS && row0 + r < a.rows;
             p[i] = there ? base + (row0 + r) * stride : nullptr;
@@ -633,24 +635,24 @@ struct Product {
     LinearJob job;
 };
 
-template <typename T> __device__ inline void write8(T* out, int64_t left, const float (&v)[8]) {
-    Values<T, 8> r;
+template <typename T, int N> __device__ inline void put_values(T* out, int64_t left, const float (&v)[N]) {
+    Values<T, N> r;
 #pragma unroll
-    for (int i = 0; i < 8; ++i) r.v[i] = static_cast<T>(v[i]);
-    if (left >= 8) {
+    for (int i = 0; i < N; ++i) r.v[i] = static_cast<T>(v[i]);
+    if (left >= N) {
         __builtin_memcpy(out, &r, sizeof(r));
     } else {
 #pragma unroll
-        for (int i = 0; i < 8; ++i) {
+        for (int i = 0; i < N; ++i) {
             if (i < left) out[i] = r.v[i];
         }
     }
 }
 
-template <typename T> __device__ inline void read8(const T* in, int64_t left, float (&v)[8]) {
-    const Values<T, 8> r = read<T, 8>(in, left);
+template <typename T, int N> __device__ inline void get_values(const T* in, int64_t left, float (&v)[N]) {
+    const Values<T, N> r = read<T, N>(in, left);
 #pragma unroll
-    for (int i = 0; i < 8; ++i) v[i] = as_float(r.v[i]);
+    for (int i = 0; i < N; ++i) v[i] = as_float(r.v[i]);
 }
 
 // Workgroup -> tile.  Workgroups are dealt to the eight XCDs in turn, so those of one XCD
@@ -671,8 +673,7 @@ __device__ inline void banded(const Product& a, int64_t tile, int64_t& row, int6
     col = in_band / rows;
 }
 
-// How a tile is shared out among wavefronts, and how much of it passes through LDS at a time
-// on its way out.
+// How a tile is shared out among wavefronts.
 template <int BR, int BC>
 struct Tile {
     static constexpr int kThreads = BR * BC >= 256 * 256 ? 512 : 256, kWaves = kThreads / 64;
@@ -680,106 +681,112 @@ struct Tile {
     static constexpr int kWaveRows = kWaves / kWaveCols;
     static constexpr int kR = BR / kWaveRows / 16, kC = BC / kWaveCols / 16;
     static constexpr int kSums = kR / kWaveCols;   // rows of P are summed by those that share them, so many of kR each
-    static constexpr int kPass = kR > 4 ? 1 : kR, kPasses = kR / kPass;   // of kR
-    static constexpr int kOutRows = kWaveRows * kPass * 16;
+    static constexpr int kOutBytes = 16 * kC * 16 * 4;   // of sixteen rows of a wavefront's columns
 };
 
 template <typename T, int BR, int BC> struct Shared {
     static constexpr int kRowBytes = Form<T>::kStep / Form<T>::kChunk * 16;
     static constexpr int kP = Form<T>::kParts * BR * kRowBytes;
     static constexpr int kQ = Form<T>::kParts * BC * kRowBytes;
-    static constexpr int kStride = BC + 4;       // floats between rows of the result
-    static constexpr int kOut = Tile<BR, BC>::kOutRows * kStride * 4;
-    static constexpr int kBytes = 2 * (kP + kQ) > kOut ? 2 * (kP + kQ) : kOut;
+    static constexpr int kBytes = 2 * (kP + kQ);
 };
 
-// The way out of a tile's sums.  They go through LDS once more, some rows of every wavefront
-// at a time, so that a thread has eight columns of a row: operands and results then come and
-// go in whole lines.
-template <typename T, typename TO, int BR, int BC, int KIND>
-__device__ inline void finish(const Product& a, char* lds, const f32x4 (&acc)[Tile<BR, BC>::kR][Tile<BR, BC>::kC],
+// The way out of a tile's sums.  Every wavefront takes sixteen rows of its own at a time
+// through LDS of its own (16-byte pieces exchanged by the row's number, so that neither way
+// meets a bank twice), after which a lane has the 16 bytes of a row next to those of its
+// neighbours: operands and results come and go in whole lines, and no wavefront waits for
+// another.  (Straight from the registers, where a lane has four columns of a row, or sixteen
+// if the columns are dealt out for that, lines go in pieces: 524 288 rows of 64 float32,
+// with slopes, 200 us for 145 by way of LDS.)
+template <typename TO, int BR, int BC, int KIND, bool SCALED>
+__device__ inline void finish(const Product& a, char* space, const f32x4 (&acc)[Tile<BR, BC>::kR][Tile<BR, BC>::kC],
                               int64_t row0, int64_t col0) {
     using W = Tile<BR, BC>;
-    constexpr int kStride = Shared<T, BR, BC>::kStride;
-    constexpr int kAcross = BC / 8, kDown = W::kThreads / kAcross;
-    constexpr int kPassRows = KIND == kLinearSecond ? W::kOutRows / 2 : W::kOutRows;
+    using Slope = typename Form<TO>::Slope;
+    constexpr bool kTwo = KIND == kLinearSecond;
+    constexpr int kTiles = kTwo ? W::kR / 2 : W::kR;
+    constexpr int N = 16 / sizeof(TO);                       // columns a lane
+    constexpr int kPieces = W::kC * 4, kLanes = W::kC * 16 / N, kDown = 64 / kLanes;
     const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
-    const int wave_col = wave % W::kWaveCols * W::kC * 16;
-    float* sums_of = reinterpret_cast<float*>(lds);
     const LinearJob& j = a.job;
-    const int at = threadIdx.x % kAcross * 8;
-    const int64_t col = col0 + at, left = a.q.rows - col;
-    float bias[8], scale[8];
+    const int64_t first_row = row0 + wave / W::kWaveCols * kTiles * 16;
+    const int at = lane % kLanes * N;
+    const int64_t col = col0 + wave % W::kWaveCols * W::kC * 16 + at, left = a.q.rows - col;
+    float bias[N], scale[N];
 #pragma unroll
-    for (int i = 0; i < 8; ++i) {
+    for (int i = 0; i < N; ++i) {
         bias[i] = 0.0f;
         scale[i] = 1.0f;
     }
-    if (j.bias != nullptr) read8(static_cast<const TO*>(j.bias) + col, left, bias);
-    if constexpr (Form<T>::kScaled) read8(j.weight_scales + col, left, scale);
+    if (j.bias != nullptr) get_values(static_cast<const TO*>(j.bias) + col, left, bias);
+    if constexpr (SCALED) get_values(j.weight_scales + col, left, scale);
+    const auto take = [&](const char* from, int r, float (&v)[N]) {
+#pragma unroll
+        for (int h = 0; h < N / 4; ++h) {
+            const int piece = (at / 4 + h) ^ (r % kPieces);
+            __builtin_memcpy(v + 4 * h, from + (r * kPieces + piece) * 16, 16);
+        }
+    };
 #pragma unroll 1
-    for (int pass = 0; pass < W::kPasses; ++pass) {
-        __syncthreads();
+    for (int n = 0; n < kTiles; ++n) {
         // (accumulators are registers: which of them is said in the code, and the rest of it is
         // there once)
 #pragma unroll
-        for (int now = 0; now < W::kPasses; ++now) {
-            if (now != pass) continue;
+        for (int now = 0; now < kTiles; ++now) {
+            if (now != n) continue;
 #pragma unroll
-            for (int r = 0; r < W::kPass; ++r) {
+            for (int two = 0; two < (kTwo ? 2 : 1); ++two) {
 #pragma unroll
                 for (int c = 0; c < W::kC; ++c) {
-                    *reinterpret_cast<f32x4*>(sums_of +
-                                              ((wave / W::kWaveCols * W::kPass + r) * 16 + (lane & 15)) * kStride +
-                                              wave_col + c * 16 + (lane >> 4) * 4) = acc[now * W::kPass + r][c];
+                    const int piece = (c * 4 + (lane >> 4)) ^ (lane % 16 % kPieces);
+                    *reinterpret_cast<f32x4*>(space + two * W::kOutBytes + (lane % 16 * kPieces + piece) * 16) =
+                            acc[kTwo ? 2 * now + two : now][c];
                 }
             }
         }
-        __syncthreads();
 #pragma unroll 1
-        for (int r = threadIdx.x / kAcross; r < kPassRows; r += kDown) {
-            // rows 16 kPass w and on of a pass are those of the wavefronts' row w
-            const int64_t row = row0 + r / (W::kPass * 16) * W::kR * 16 + pass * W::kPass * 16 + r % (W::kPass * 16);
+        for (int r = lane / kLanes; r < 16; r += kDown) {
+            const int64_t row = first_row + n * 16 + r;
             if (row >= a.p.rows || left <= 0) continue;
-            float z[8], y[8], d[8];
-            const float row_scale = Form<T>::kScaled ? j.input_scales[row] : 1.0f;
+            float z[N], y[N], d[N];
+            take(space, r, z);
+            const float row_scale = SCALED ? j.input_scales[row] : 1.0f;
 #pragma unroll
-            for (int i = 0; i < 8; ++i) {
-                z[i] = sums_of[r * kStride + at + i];
-                if constexpr (Form<T>::kScaled) z[i] *= row_scale * scale[i];
+            for (int i = 0; i < N; ++i) {
+                if constexpr (SCALED) z[i] *= row_scale * scale[i];
                 z[i] += bias[i];
             }
             const int64_t o = row * a.q.rows + col;
-            if constexpr (KIND == kLinearSecond) {
+            if constexpr (kTwo) {
                 // t: the derivative of <second input, gradient of the input> by gz
-                float t[8], g[8], dd[8];
-#pragma unroll
-                for (int i = 0; i < 8; ++i) t[i] = sums_of[(kPassRows + r) * kStride + at + i];
+                float t[N], g[N], dd[N];
+                take(space + W::kOutBytes, r, t);
                 if (j.addend != nullptr) {
-                    float more[8];
-                    read8(static_cast<const TO*>(j.addend) + row * j.addend_stride + col, left, more);
+                    get_values(static_cast<const TO*>(j.addend) + row * j.addend_stride + col, left, g);
 #pragma unroll
-                    for (int i = 0; i < 8; ++i) t[i] += more[i];
+                    for (int i = 0; i < N; ++i) t[i] += g[i];
                 }
-                read8(static_cast<const TO*>(j.grad) + o, left, g);
+                get_values(static_cast<const TO*>(j.grad) + o, left, g);
                 curve(j.activation, j.act_scale, z, d, dd);
 #pragma unroll
-                for (int i = 0; i < 8; ++i) {
+                for (int i = 0; i < N; ++i) {
                     y[i] = t[i] * d[i];
                     dd[i] *= t[i] * g[i];
                 }
-                if (j.out != nullptr) write8(static_cast<TO*>(j.out) + o, left, y);
-                if (j.curvature_out != nullptr) write8(static_cast<TO*>(j.curvature_out) + o, left, dd);
+                if (j.out != nullptr) put_values(static_cast<TO*>(j.out) + o, left, y);
+                if (j.curvature_out != nullptr) put_values(static_cast<TO*>(j.curvature_out) + o, left, dd);
             } else {
+                float more[N];
+                if (j.residual != nullptr) {
+                    get_values(static_cast<const TO*>(j.residual) + row * j.residual_stride + col, left, more);
+                }
                 activate(j.activation, j.act_scale, z, y, d);
                 if (j.residual != nullptr) {
-                    float more[8];
-                    read8(static_cast<const TO*>(j.residual) + row * j.residual_stride + col, left, more);
 #pragma unroll
-                    for (int i = 0; i < 8; ++i) y[i] += more[i];
+                    for (int i = 0; i < N; ++i) y[i] += more[i];
                 }
-                write8(static_cast<TO*>(j.out) + o, left, y);
-                if (j.slope_out != nullptr) write8(static_cast<typename Form<TO>::Slope*>(j.slope_out) + o, left, d);
+                put_values(static_cast<TO*>(j.out) + o, left, y);
+                if (j.slope_out != nullptr) put_values(static_cast<Slope*>(j.slope_out) + o, left, d);
             }
         }
     }
@@ -852,6 +859,7 @@ __global__ __launch_bounds__((Tile<BR, BC>::kThreads)) void product_kernel(const
     constexpr bool kGrad = KIND == kLinearGradInput || KIND == kLinearGradWeight;
     constexpr int kStep = Form<T>::kStep;
     __shared__ __attribute__((aligned(16))) char lds[S::kBytes];
+    static_assert(W::kWaves * W::kOutBytes * (KIND == kLinearSecond ? 2 : 1) <= S::kBytes, "");
 
     Place w;
     if (!place_of<KIND>(a, w)) return;
@@ -931,7 +939,9 @@ __global__ __launch_bounds__((Tile<BR, BC>::kThreads)) void product_kernel(const
     if constexpr (KIND == kLinearGradWeight) {
         leave_part<BR, BC>(a, acc, rows_sum, w.part, row0, col0, w.sums);
     } else {
-        finish<T, TO, BR, BC, KIND>(a, lds, acc, row0, col0);
+        __syncthreads();   // of all wavefronts' reads of their operands
+        finish<TO, BR, BC, KIND, Form<T>::kScaled>(a, lds + wave * W::kOutBytes * (KIND == kLinearSecond ? 2 : 1), acc,
+                                                   row0, col0);
     }
 }
 
@@ -1185,12 +1195,11 @@ template <typename T, typename TO, int KIND>
 __global__ __launch_bounds__(kLargeThreads) void large_kernel(const Product a) {
     constexpr bool kStackP = KIND == kLinearGradWeight, kStackQ = KIND != kLinearForward;
     using Work = LargeWork<T, kStackP, kStackQ>;
-    constexpr int kOut = LargeTile::kOutRows * (kLarge + 4) * 4;
+    static_assert(4 * LargeTile::kOutBytes <= Work::kP && 4 * LargeTile::kOutBytes <= Work::kQ, "");
     constexpr bool kFour = Stage<T>::kStages > 2;
     // Planes under names of their own: the compiler then sees that reads of one need not wait
     // for loads into another (it looks only so far through an address, hence one each).
-    __shared__ __attribute__((aligned(16))) char p0[Work::kP > kOut ? Work::kP : kOut];
-    __shared__ __attribute__((aligned(16))) char p1[Work::kP], p2[kFour ? Work::kP : 16], p3[kFour ? Work::kP : 16];
+    __shared__ __attribute__((aligned(16))) char p0[Work::kP], p1[Work::kP], p2[kFour ? Work::kP : 16], p3[kFour ? Work::kP : 16];
     __shared__ __attribute__((aligned(16))) char q0[Work::kQ], q1[Work::kQ], q2[kFour ? Work::kQ : 16],
             q3[kFour ? Work::kQ : 16];
 
@@ -1205,7 +1214,9 @@ __global__ __launch_bounds__(kLargeThreads) void large_kernel(const Product a) {
         leave_part<kLarge, kLarge>(a, work.acc, work.rows_sum, w.part, row0, col0, w.sums);
     } else {
         work.template run<false>({p0, q0}, {p1, q1}, {p2, q2}, {p3, q3});
-        finish<T, TO, kLarge, kLarge, KIND>(a, p0, work.acc, row0, col0);
+        __syncthreads();   // of all wavefronts' reads of their operands
+        char* space = (work.wave < 4 ? p0 : q0) + work.wave % 4 * LargeTile::kOutBytes;
+        finish<TO, kLarge, kLarge, KIND, Form<T>::kScaled>(a, space, work.acc, row0, col0);
     }
 }
 
