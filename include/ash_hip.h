@@ -965,11 +965,15 @@ typedef struct ash_linear_args {
     int64_t input_stride, residual_stride;
     int32_t dtype, out_dtype, activation;
     float activation_scale;
+    int32_t slope_is_output;     /* backward calls: slope is the output, see below */
 } ash_linear_args;
 
 /* slope: f'(z) for the backward calls, or NULL; float32, for ASH_BF16 float16, and
  * of SINE without its factor a. */
 int ash_linear_forward(const ash_linear_args* args, void* output, void* slope, void* stream);
+/* 1: the output, if it has no residual, tells the slope; the backward calls take it as
+ * slope with slope_is_output set, and the forward need not leave another. */
+int ash_linear_slope_by_output(int32_t dtype, int32_t activation);
 /* grad_input = (grad * slope) weight (+ addend); slope NULL: f'(z) is one.  Reads
  * weight, the activation (whose factor a slope is without) and the sizes of args. */
 int ash_linear_backward_input(const ash_linear_args* args, const void* grad, const void* slope,

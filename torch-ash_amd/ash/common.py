@@ -73,6 +73,7 @@ class _LinearArgs(ctypes.Structure):
         ("out_dtype", ctypes.c_int32),
         ("activation", ctypes.c_int32),
         ("activation_scale", ctypes.c_float),
+        ("slope_is_output", ctypes.c_int32),
     ]
 
 
@@ -381,6 +382,7 @@ _SIGNATURES = {
     ),
     "ash_linear_forward": (ctypes.c_int, [ctypes.POINTER(_LinearArgs), _PTR, _PTR, _PTR]),
     "ash_linear_backward_input": (ctypes.c_int, [ctypes.POINTER(_LinearArgs)] + [_PTR] * 5),
+    "ash_linear_slope_by_output": (ctypes.c_int, [ctypes.c_int32, ctypes.c_int32]),
     "ash_linear_wants_scaled_gradient": (ctypes.c_int, [_I64, _I64, _I64, ctypes.c_int32]),
     "ash_linear_scale_gradient": (ctypes.c_int, [ctypes.POINTER(_LinearArgs)] + [_PTR] * 4),
     "ash_linear_backward_weight_scratch_bytes": (

@@ -73,6 +73,7 @@ namespace py = pybind11;
     X(ash_query_backward_backward_scaled)                                             \
     X(ash_linear_forward)                                                             \
     X(ash_linear_backward_input)                                                      \
+    X(ash_linear_slope_by_output)                                                     \
     X(ash_linear_wants_scaled_gradient)                                               \
     X(ash_linear_scale_gradient)                                                      \
     X(ash_linear_backward_weight_scratch_bytes)                                       \
@@ -1030,6 +1031,7 @@ std::vector<int64_t> shape_with(const Tensor& input, int64_t width) {
 struct Activation {
     int32_t kind;
     double scale;
+    bool by_output = false;   // the kept slope is the output
     bool curved() const { return kind != ASH_ACT_NONE && kind != ASH_ACT_RELU; }
 };
 
@@ -1045,6 +1047,7 @@ ash_linear_args linear_args(const Tensor& x, const Tensor& w, const Tensor& b, c
     a.dtype = a.out_dtype = layer_dtype(x, "input");
     a.activation = f.kind;
     a.activation_scale = static_cast<float>(f.scale);
+    a.slope_is_output = f.by_output;
     return a;
 }
 
@@ -1091,6 +1094,7 @@ Tensor linear_backward_input(const Tensor& grad, const Tensor& slope, const Tens
     a.dtype = a.out_dtype = layer_dtype(grad, "grad");
     a.activation = f.kind;
     a.activation_scale = static_cast<float>(f.scale);
+    a.slope_is_output = f.by_output;
     Tensor out = empty({a.rows, a.in_features}, grad.scalar_type(), device);
     check(lib.ash_linear_backward_input(&a, grad.data_ptr(), ptr<void>(slope), ptr<void>(addend), out.data_ptr(),
                                         stream_of(device)));
@@ -1117,6 +1121,7 @@ std::pair<Tensor, Tensor> linear_backward_weight(const Pair& one, const Pair& tw
     a.dtype = a.out_dtype = layer_dtype(grad, "grad");
     a.activation = f.kind;
     a.activation_scale = static_cast<float>(f.scale);
+    a.slope_is_output = f.by_output;
     const Tensor gw = need_weight ? empty({a.out_features, a.in_features}, grad.scalar_type(), device) : Tensor();
     const Tensor gb = need_bias ? empty({a.out_features}, grad.scalar_type(), device) : Tensor();
     const int64_t bytes = lib.ash_linear_backward_weight_scratch_bytes(a.rows, a.in_features, a.out_features, a.dtype,
@@ -1150,11 +1155,12 @@ void leaves_may_be_captured(std::initializer_list<const Tensor*> tensors) {
 // that are), hence the optionals, and it returns the gradients that are asked for only.
 struct LinearGrad : torch::autograd::Function<LinearGrad> {
     static variable_list forward(AutogradContext* ctx, const Tensor& grad_in, const Tensor& x_in, const Tensor& w_in,
-                                 const Optional& b, const Optional& slope, int64_t kind, double scale, bool need_x,
-                                 bool need_w, bool need_b) {
+                                 const Optional& b, const Optional& slope, int64_t kind, double scale, bool by_output,
+                                 bool need_x, bool need_w, bool need_b) {
         const Tensor grad = grad_in.contiguous(), x = readable(x_in), w = w_in.contiguous();
         const Tensor d = slope.value_or(Tensor());
-        const Activation f{static_cast<int32_t>(kind), scale};
+        const Activation f{static_cast<int32_t>(kind), scale, by_output};
+        ctx->saved_data["by_output"] = by_output;
         ctx->save_for_backward({grad_in, x_in, w_in, b.value_or(Tensor()), d});
         ctx->saved_data["kind"] = kind;
         ctx->saved_data["scale"] = scale;
@@ -1175,7 +1181,8 @@ struct LinearGrad : torch::autograd::Function<LinearGrad> {
         const auto saved = ctx->get_saved_variables();
         const Tensor grad = saved[0].contiguous(), x = readable(saved[1]), w = saved[2].contiguous();
         const Tensor b = saved[3].defined() ? saved[3].contiguous() : Tensor(), d = saved[4];
-        const Activation f{static_cast<int32_t>(ctx->saved_data["kind"].toInt()), ctx->saved_data["scale"].toDouble()};
+        const Activation f{static_cast<int32_t>(ctx->saved_data["kind"].toInt()), ctx->saved_data["scale"].toDouble(),
+                           ctx->saved_data["by_output"].toBool()};
         const int64_t needs = ctx->saved_data["needs"].toInt();
         size_t next = 0;
         const auto take = [&](int64_t bit) {
@@ -1183,7 +1190,7 @@ struct LinearGrad : torch::autograd::Function<LinearGrad> {
             return t.defined() ? t.contiguous() : t;
         };
         const Tensor u = take(1), of_w = take(2), of_b = take(4);
-        variable_list out(10);
+        variable_list out(11);
         if (!u.defined() && !of_w.defined() && !of_b.defined()) return out;
         const bool need_grad = ctx->needs_input_grad(0), need_x = ctx->needs_input_grad(1),
                    need_w = ctx->needs_input_grad(2), need_b = b.defined() && ctx->needs_input_grad(3);
@@ -1225,12 +1232,14 @@ struct Linear : torch::autograd::Function<Linear> {
                           const Optional& residual, int64_t kind, double scale) {
         const Tensor x = readable(x_in), w = w_in.contiguous();
         const Tensor b = b_in.has_value() ? b_in->contiguous() : Tensor();
-        const Activation f{static_cast<int32_t>(kind), scale};
+        Activation f{static_cast<int32_t>(kind), scale};
         const bool learns = x_in.requires_grad() || w_in.requires_grad() || (b_in.has_value() && b_in->requires_grad());
+        const bool by_output = !residual.has_value() && lib.ash_linear_slope_by_output(layer_dtype(x, "input"), f.kind);
         Tensor slope;
         const Tensor out = linear_forward(x, w, b, residual.has_value() ? readable(*residual) : Tensor(), f,
-                                          learns && kind != ASH_ACT_NONE ? &slope : nullptr);
-        ctx->save_for_backward({x_in, w_in, b_in.value_or(Tensor()), slope});
+                                          learns && kind != ASH_ACT_NONE && !by_output ? &slope : nullptr);
+        ctx->save_for_backward({x_in, w_in, b_in.value_or(Tensor()), learns && by_output ? out : slope});
+        ctx->saved_data["by_output"] = by_output;
         ctx->saved_data["kind"] = kind;
         ctx->saved_data["scale"] = scale;
         ctx->saved_data["residual"] = residual.has_value();
@@ -1242,14 +1251,16 @@ struct Linear : torch::autograd::Function<Linear> {
         variable_list out(6);
         if (!grads[0].defined()) return out;
         const auto saved = ctx->get_saved_variables();
-        const Tensor &x = saved[0], &w = saved[1], &b = saved[2], &slope = saved[3];
+        const Tensor &x = saved[0], &w = saved[1], &b = saved[2];
+        const Tensor slope = saved[3].defined() ? saved[3].detach() : Tensor();
+        const bool by_output = ctx->saved_data["by_output"].toBool();
         const bool need_x = ctx->needs_input_grad(0), need_w = ctx->needs_input_grad(1),
                    need_b = b.defined() && ctx->needs_input_grad(2);
         if (ctx->saved_data["residual"].toBool() && ctx->needs_input_grad(b.defined() ? 3 : 2)) out[3] = grads[0];
         if (!need_x && !need_w && !need_b) return out;
         if (at::GradMode::is_enabled()) {
             const auto got = LinearGrad::apply(grads[0], x, w, maybe(b), maybe(slope), ctx->saved_data["kind"].toInt(),
-                                               ctx->saved_data["scale"].toDouble(), need_x, need_w, need_b);
+                                               ctx->saved_data["scale"].toDouble(), by_output, need_x, need_w, need_b);
             size_t next = 0;
             if (need_x) out[0] = got[next++];
             if (need_w) out[1] = got[next++];
@@ -1257,7 +1268,8 @@ struct Linear : torch::autograd::Function<Linear> {
             return out;
         }
         Tensor grad = grads[0].contiguous(), d = slope;
-        const Activation f{static_cast<int32_t>(ctx->saved_data["kind"].toInt()), ctx->saved_data["scale"].toDouble()};
+        const Activation f{static_cast<int32_t>(ctx->saved_data["kind"].toInt()), ctx->saved_data["scale"].toDouble(),
+                           by_output};
         if (need_x && need_w) scale_gradient(grad, d, x, w, f);
         if (need_x) out[0] = linear_backward_input(grad, d, w.contiguous(), Tensor(), f);
         if (need_w || need_b) {
@@ -1382,6 +1394,7 @@ Tensor linear_quantized(const Tensor& x, const Tensor& x_scales, const Tensor& w
     a.out_dtype = type == at::kFloat ? ASH_F32 : type == at::kHalf ? ASH_F16 : ASH_BF16;
     a.activation = f.kind;
     a.activation_scale = static_cast<float>(f.scale);
+    a.slope_is_output = f.by_output;
     Tensor out = empty(shape, type, device);
     check(lib.ash_linear_forward(&a, out.data_ptr(), nullptr, stream_of(device)));
     return out;

@@ -512,6 +512,9 @@ int check_linear(const ash_linear_args* a, bool eight_bits, const char* what) {
     if (!(a->activation_scale > 0.0f) || a->activation_scale > 3.4028235e38f) {
         ASH_FAIL("linear: the activation's scale must be positive and finite");
     }
+    if (a->slope_is_output && !ash_linear_slope_by_output(a->dtype, a->activation)) {
+        ASH_FAIL(std::string(what) + ": the output does not tell the slope");
+    }
     if (a->rows > 0 && (a->input == nullptr || a->weight == nullptr ||
                         (a->dtype == ASH_E4M3 && (a->input_scales == nullptr || a->weight_scales == nullptr)))) {
         ASH_FAIL(std::string("null pointer in ") + what);
@@ -538,6 +541,10 @@ LinearJob job_of(const ash_linear_args& a) {
     j.act_scale = a.activation_scale;
     j.splits = 1;
     j.slope_factor = a.activation == ASH_ACT_SINE ? a.activation_scale : 1.0f;
+    if (a.slope_is_output) {
+        j.slope_kind = a.activation == ASH_ACT_RELU ? 1 : 2;
+        if (a.activation == ASH_ACT_SOFTPLUS) j.slope_factor = a.activation_scale;
+    }
     return j;
 }
 
@@ -589,6 +596,10 @@ int ash_linear_backward_input(const ash_linear_args* args, const void* grad, con
     PointerGuard guard;
     ASH_HIP(guard.enter_for(grad));
     return run_linear(kLinearGradInput, j, args->dtype, static_cast<hipStream_t>(stream));
+}
+
+int ash_linear_slope_by_output(int32_t dtype, int32_t activation) {
+    return dtype == ASH_F32 && (activation == ASH_ACT_RELU || activation == ASH_ACT_SOFTPLUS);
 }
 
 int ash_linear_wants_scaled_gradient(int64_t rows, int64_t in_features, int64_t out_features, int32_t dtype) {

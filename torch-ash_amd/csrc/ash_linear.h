@@ -21,6 +21,7 @@ struct LinearJob {
     const void* grad;         // gradients only: of the output
     const void* slope;        // f'(z) / slope_factor as the forward left it, or null: one
     float slope_factor;
+    int32_t slope_kind;       // ash_linear.hip: SlopeKind
     const float* input_scales;
     const float* weight_scales;
     void* out;

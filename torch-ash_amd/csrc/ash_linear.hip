@@ -142,6 +142,7 @@ struct Side {
     int64_t stride;     // values between rows (lying along k) or between values of k
     int64_t rows;
     float factor;       // of mul
+    int32_t kind;       // SlopeKind
 };
 
 template <typename T> __device__ inline uint4 packed(const float (&v)[8]) {
@@ -151,6 +152,32 @@ template <typename T> __device__ inline uint4 packed(const float (&v)[8]) {
     uint4 u;
     __builtin_memcpy(&u, &r, 16);
     return u;
+}
+
+// exp(x) by the unit's exp2: the argument's product with log2(e) in two parts, of which the
+// second, below a step of the first, is applied as a factor.
+__device__ inline float exp_of(float x) {
+    const float t = x * 1.44269504f;
+    const float rest = fmaf(x, 1.44269504f, -t) + x * 1.92596299e-8f;
+    const float e = __builtin_amdgcn_exp2f(t);
+    // (beyond the range of float the first part says all there is)
+    return fabsf(rest) < 1.0f ? fmaf(e, rest * 0.69314718f, e) : e;
+}
+
+// f'(z) / factor by what was kept: itself, or (float32 alone) the output of an activation that
+// tells it, without a residual: 0 or more of relu, log(1 + exp(a z)) / a of softplus, whose
+// slope is 1 - exp(-a y).
+enum SlopeKind { kSlopeKept, kSlopeRelu, kSlopeSoftplus };
+template <typename T> __device__ inline float slope_of(float kept, int kind, float factor) {
+    if constexpr (sizeof(T) == 4) {
+        if (kind == kSlopeRelu) return kept > 0.0f ? 1.0f : 0.0f;
+        if (kind == kSlopeSoftplus) {
+            const float t = factor * kept;   // (the factor is a)
+            const float near = t * fmaf(t, fmaf(t, fmaf(t, -0.041666668f, 0.16666667f), -0.5f), 1.0f);
+            return t < 0.03125f ? near : 1.0f - exp_of(-t);
+        }
+    }
+    return factor * kept;
 }
 
 // Eight consecutive values of k of one row into LDS.
@@ -184,6 +211,7 @@ struct Along {
     int row[kEach], chunk;
     bool mul;
     float factor;
+    int kind;
     Values<T, N> v[kEach];
     Values<M, N> w[kEach];
 
@@ -194,6 +222,7 @@ struct Along {
         chunk = threadIdx.x % kChunks;
         mul = MUL && a.mul != nullptr;
         factor = a.factor;
+        kind = a.kind;
 #pragma unroll
         for (int i = 0; i < kEach; ++i) {
             row[i] = (threadIdx.x + i * THREADS) / kChunks;
@@ -235,7 +264,7 @@ struct Along {
                 if constexpr (MUL) {
                     if (mul) {
 #pragma unroll
-                        for (int j = 0; j < 8; ++j) f[j] *= factor * as_float(w[i].v[j]);
+                        for (int j = 0; j < 8; ++j) f[j] *= slope_of<T>(as_float(w[i].v[j]), kind, factor);
                     }
                 }
                 put<T, ROWS>(plane, row[i], chunk, f);
@@ -261,6 +290,7 @@ struct Across {
     int row, group;
     bool mul, works;
     float factor;
+    int kind;
     Values<T, kWide> v[8];
     Values<typename Form<T>::Slope, kWide> w[8];
 
@@ -274,6 +304,7 @@ struct Across {
         mul = MUL && a.mul != nullptr;
         p = static_cast<const T*>(a.p) + row0 + row;
         factor = a.factor;
+        kind = a.kind;
         m = mul ? static_cast<const typename Form<T>::Slope*>(a.mul) + row0 + row : nullptr;
     }
     __device__ void load(int64_t k0, int64_t k_end) {
@@ -296,7 +327,7 @@ struct Across {
             for (int j = 0; j < 8; ++j) {
                 f[j] = as_float(v[j].v[i]);
                 if constexpr (MUL) {
-                    if (mul) f[j] *= factor * as_float(w[j].v[i]);
+                    if (mul) f[j] *= slope_of<T>(as_float(w[j].v[i]), kind, factor);
                 }
             }
             put<T, ROWS>(plane, row + i, group, f);
@@ -318,6 +349,7 @@ struct Stacked {
     int chunk;
     bool mul;
     float factor;
+    int kind;
     Values<T, 8> v[kEach];
     Values<M, 8> w[kEach];
 
@@ -328,6 +360,7 @@ struct Stacked {
         left = a.rows - (row0 + chunk * 8);
         mul = MUL && a.mul != nullptr;
         factor = a.factor;
+        kind = a.kind;
         p = static_cast<const T*>(a.p) + row0 + chunk * 8;
         m = mul ? static_cast<const M*>(a.mul) + row0 + chunk * 8 : nullptr;
     }
@@ -352,7 +385,7 @@ struct Stacked {
                 if (mul) {
                     float f[8];
 #pragma unroll
-                    for (int j = 0; j < 8; ++j) f[j] = as_float(v[i].v[j]) * (factor * as_float(w[i].v[j]));
+                    for (int j = 0; j < 8; ++j) f[j] = as_float(v[i].v[j]) * slope_of<T>(as_float(w[i].v[j]), kind, factor);
                     u = packed<T>(f);
                 }
             }
@@ -449,16 +482,6 @@ __device__ inline f32x4 sum_rows(const Fragment<float>& p, f32x4 c) {
 }
 
 // --------------------------------------------------------------------- activations
-// exp(x) by the unit's exp2: the argument's product with log2(e) in two parts, of which the
-// second, below a step of the first, is applied as a factor.
-__device__ inline float exp_of(float x) {
-    const float t = x * 1.44269504f;
-    const float rest = fmaf(x, 1.44269504f, -t) + x * 1.92596299e-8f;
-    const float e = __builtin_amdgcn_exp2f(t);
-    // (beyond the range of float the first part says all there is)
-    return fabsf(rest) < 1.0f ? fmaf(e, rest * 0.69314718f, e) : e;
-}
-
 __device__ inline float sigmoid(float v) { return __builtin_amdgcn_rcpf(1.0f + exp_of(-v)); }
 
 // The normal distribution's integral and its density at z.  The complementary error function
@@ -635,12 +658,21 @@ struct Product {
     LinearJob job;
 };
 
-template <typename T, int N> __device__ inline void put_values(T* out, int64_t left, const float (&v)[N]) {
+// STREAM: past the caches (of the large tiles' outputs, which fill them several times over,
+// 65 536 rows of 1024 bf16: 171 -> 158 us).
+template <typename T, int N, bool STREAM> __device__ inline void put_values(T* out, int64_t left, const float (&v)[N]) {
+    typedef uint32_t Word __attribute__((ext_vector_type(N * sizeof(T) / 4), aligned(2)));
     Values<T, N> r;
 #pragma unroll
     for (int i = 0; i < N; ++i) r.v[i] = static_cast<T>(v[i]);
     if (left >= N) {
-        __builtin_memcpy(out, &r, sizeof(r));
+        if constexpr (STREAM) {
+            Word w;
+            __builtin_memcpy(&w, &r, sizeof(r));
+            __builtin_nontemporal_store(w, reinterpret_cast<Word*>(out));
+        } else {
+            __builtin_memcpy(out, &r, sizeof(r));
+        }
     } else {
 #pragma unroll
         for (int i = 0; i < N; ++i) {
@@ -691,62 +723,57 @@ template <typename T, int BR, int BC> struct Shared {
     static constexpr int kBytes = 2 * (kP + kQ);
 };
 
-// The way out of a tile's sums.  Every wavefront takes sixteen rows of its own at a time
-// through LDS of its own (16-byte pieces exchanged by the row's number, so that neither way
-// meets a bank twice), after which a lane has the 16 bytes of a row next to those of its
-// neighbours: operands and results come and go in whole lines, and no wavefront waits for
-// another.  (Straight from the registers, where a lane has four columns of a row, or sixteen
-// if the columns are dealt out for that, lines go in pieces: 524 288 rows of 64 float32,
-// with slopes, 200 us for 145 by way of LDS.)
-template <typename TO, int BR, int BC, int KIND, bool SCALED>
-__device__ inline void finish(const Product& a, char* space, const f32x4 (&acc)[Tile<BR, BC>::kR][Tile<BR, BC>::kC],
-                              int64_t row0, int64_t col0) {
-    using W = Tile<BR, BC>;
+// The way out of sixteen rows of a wavefront's sums (two sets of them for the second order).
+// They go through LDS of the wavefront's own (16-byte pieces exchanged by the row's number, so
+// that neither way meets a bank twice), after which a lane has the 16 bytes of a row next to
+// those of its neighbours: operands and results come and go in whole lines, and no wavefront
+// waits for another.  (Straight from the registers, where a lane has four columns of a row, or
+// sixteen if the columns are dealt out for that, lines go in pieces: 524 288 rows of 64
+// float32, with slopes, 200 us for 145 by way of LDS.)
+template <typename TO, int KC, int KIND, bool SCALED, bool STREAM>
+struct Finish {
     using Slope = typename Form<TO>::Slope;
-    constexpr bool kTwo = KIND == kLinearSecond;
-    constexpr int kTiles = kTwo ? W::kR / 2 : W::kR;
-    constexpr int N = 16 / sizeof(TO);                       // columns a lane
-    constexpr int kPieces = W::kC * 4, kLanes = W::kC * 16 / N, kDown = 64 / kLanes;
-    const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
-    const LinearJob& j = a.job;
-    const int64_t first_row = row0 + wave / W::kWaveCols * kTiles * 16;
-    const int at = lane % kLanes * N;
-    const int64_t col = col0 + wave % W::kWaveCols * W::kC * 16 + at, left = a.q.rows - col;
+    static constexpr bool kTwo = KIND == kLinearSecond;
+    static constexpr int N = 16 / sizeof(TO);                       // columns a lane
+    static constexpr int kPieces = KC * 4, kLanes = KC * 16 / N, kDown = 64 / kLanes;
+    static constexpr int kBytes = 16 * KC * 16 * 4;
+    int lane, at;
+    int64_t col, left;
     float bias[N], scale[N];
+
+    // col0: of the wavefront
+    __device__ void start(const Product& a, int64_t col0) {
+        lane = threadIdx.x & 63;
+        at = lane % kLanes * N;
+        col = col0 + at;
+        left = a.q.rows - col;
 #pragma unroll
-    for (int i = 0; i < N; ++i) {
-        bias[i] = 0.0f;
-        scale[i] = 1.0f;
+        for (int i = 0; i < N; ++i) {
+            bias[i] = 0.0f;
+            scale[i] = 1.0f;
+        }
+        if (a.job.bias != nullptr) get_values(static_cast<const TO*>(a.job.bias) + col, left, bias);
+        if constexpr (SCALED) get_values(a.job.weight_scales + col, left, scale);
     }
-    if (j.bias != nullptr) get_values(static_cast<const TO*>(j.bias) + col, left, bias);
-    if constexpr (SCALED) get_values(j.weight_scales + col, left, scale);
-    const auto take = [&](const char* from, int r, float (&v)[N]) {
+    __device__ void give(char* space, const f32x4 (&acc)[KC], int set = 0) const {
+#pragma unroll
+        for (int c = 0; c < KC; ++c) {
+            const int piece = (c * 4 + (lane >> 4)) ^ (lane % 16 % kPieces);
+            *reinterpret_cast<f32x4*>(space + set * kBytes + (lane % 16 * kPieces + piece) * 16) = acc[c];
+        }
+    }
+    __device__ void take(const char* from, int r, float (&v)[N]) const {
 #pragma unroll
         for (int h = 0; h < N / 4; ++h) {
             const int piece = (at / 4 + h) ^ (r % kPieces);
             __builtin_memcpy(v + 4 * h, from + (r * kPieces + piece) * 16, 16);
         }
-    };
-#pragma unroll 1
-    for (int n = 0; n < kTiles; ++n) {
-        // (accumulators are registers: which of them is said in the code, and the rest of it is
-        // there once)
-#pragma unroll
-        for (int now = 0; now < kTiles; ++now) {
-            if (now != n) continue;
-#pragma unroll
-            for (int two = 0; two < (kTwo ? 2 : 1); ++two) {
-#pragma unroll
-                for (int c = 0; c < W::kC; ++c) {
-                    const int piece = (c * 4 + (lane >> 4)) ^ (lane % 16 % kPieces);
-                    *reinterpret_cast<f32x4*>(space + two * W::kOutBytes + (lane % 16 * kPieces + piece) * 16) =
-                            acc[kTwo ? 2 * now + two : now][c];
-                }
-            }
-        }
+    }
+    __device__ void rows(const Product& a, const char* space, int64_t first_row) const {
+        const LinearJob& j = a.job;
 #pragma unroll 1
         for (int r = lane / kLanes; r < 16; r += kDown) {
-            const int64_t row = first_row + n * 16 + r;
+            const int64_t row = first_row + r;
             if (row >= a.p.rows || left <= 0) continue;
             float z[N], y[N], d[N];
             take(space, r, z);
@@ -760,7 +787,7 @@ __device__ inline void finish(const Product& a, char* space, const f32x4 (&acc)[
             if constexpr (kTwo) {
                 // t: the derivative of <second input, gradient of the input> by gz
                 float t[N], g[N], dd[N];
-                take(space + W::kOutBytes, r, t);
+                take(space + kBytes, r, t);
                 if (j.addend != nullptr) {
                     get_values(static_cast<const TO*>(j.addend) + row * j.addend_stride + col, left, g);
 #pragma unroll
@@ -773,8 +800,8 @@ __device__ inline void finish(const Product& a, char* space, const f32x4 (&acc)[
                     y[i] = t[i] * d[i];
                     dd[i] *= t[i] * g[i];
                 }
-                if (j.out != nullptr) put_values(static_cast<TO*>(j.out) + o, left, y);
-                if (j.curvature_out != nullptr) put_values(static_cast<TO*>(j.curvature_out) + o, left, dd);
+                if (j.out != nullptr) put_values<TO, N, STREAM>(static_cast<TO*>(j.out) + o, left, y);
+                if (j.curvature_out != nullptr) put_values<TO, N, STREAM>(static_cast<TO*>(j.curvature_out) + o, left, dd);
             } else {
                 float more[N];
                 if (j.residual != nullptr) {
@@ -785,10 +812,35 @@ __device__ inline void finish(const Product& a, char* space, const f32x4 (&acc)[
 #pragma unroll
                     for (int i = 0; i < N; ++i) y[i] += more[i];
                 }
-                put_values(static_cast<TO*>(j.out) + o, left, y);
-                if (j.slope_out != nullptr) put_values(static_cast<Slope*>(j.slope_out) + o, left, d);
+                put_values<TO, N, STREAM>(static_cast<TO*>(j.out) + o, left, y);
+                if (j.slope_out != nullptr) put_values<Slope, N, STREAM>(static_cast<Slope*>(j.slope_out) + o, left, d);
             }
         }
+    }
+};
+
+// The same of all of a wavefront's rows of a tile.
+template <typename TO, int BR, int BC, int KIND, bool SCALED, bool STREAM>
+__device__ inline void finish(const Product& a, char* space, const f32x4 (&acc)[Tile<BR, BC>::kR][Tile<BR, BC>::kC],
+                              int64_t row0, int64_t col0) {
+    using W = Tile<BR, BC>;
+    constexpr bool kTwo = KIND == kLinearSecond;
+    constexpr int kTiles = kTwo ? W::kR / 2 : W::kR;
+    const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+    Finish<TO, W::kC, KIND, SCALED, STREAM> out;
+    out.start(a, col0 + wave % W::kWaveCols * W::kC * 16);
+    const int64_t first_row = row0 + wave / W::kWaveCols * kTiles * 16;
+#pragma unroll 1
+    for (int n = 0; n < kTiles; ++n) {
+        // (accumulators are registers: which of them is said in the code, and the rest of it is
+        // there once)
+#pragma unroll
+        for (int now = 0; now < kTiles; ++now) {
+            if (now != n) continue;
+            out.give(space, acc[kTwo ? 2 * now : now]);
+            if constexpr (kTwo) out.give(space, acc[2 * now + 1], 1);
+        }
+        out.rows(a, space, first_row + n * 16);
     }
 }
 
@@ -940,7 +992,7 @@ __global__ __launch_bounds__((Tile<BR, BC>::kThreads)) void product_kernel(const
         leave_part<BR, BC>(a, acc, rows_sum, w.part, row0, col0, w.sums);
     } else {
         __syncthreads();   // of all wavefronts' reads of their operands
-        finish<TO, BR, BC, KIND, Form<T>::kScaled>(a, lds + wave * W::kOutBytes * (KIND == kLinearSecond ? 2 : 1), acc,
+        finish<TO, BR, BC, KIND, Form<T>::kScaled, false>(a, lds + wave * W::kOutBytes * (KIND == kLinearSecond ? 2 : 1), acc,
                                                    row0, col0);
     }
 }
@@ -1216,7 +1268,7 @@ __global__ __launch_bounds__(kLargeThreads) void large_kernel(const Product a) {
         work.template run<false>({p0, q0}, {p1, q1}, {p2, q2}, {p3, q3});
         __syncthreads();   // of all wavefronts' reads of their operands
         char* space = (work.wave < 4 ? p0 : q0) + work.wave % 4 * LargeTile::kOutBytes;
-        finish<TO, kLarge, kLarge, KIND, Form<T>::kScaled>(a, space, work.acc, row0, col0);
+        finish<TO, kLarge, kLarge, KIND, Form<T>::kScaled, true>(a, space, work.acc, row0, col0);
     }
 }
 
@@ -1227,8 +1279,7 @@ constexpr int kFewThreads = 512;
 constexpr int kFewWaves = kFewThreads / 64;
 constexpr int kAhead = 4;   // steps whose operands are on their way at a time
 
-template <typename T> __device__ inline Fragment<T> direct(const T* p, int64_t left) {
-    const Values<T, Form<T>::kLane> v = read<T, Form<T>::kLane>(p, left);
+template <typename T> __device__ inline Fragment<T> formed(const Values<T, Form<T>::kLane>& v) {
     Fragment<T> f;
     if constexpr (Form<T>::kParts == 3) {
         const Three t = split(v.v);
@@ -1259,8 +1310,8 @@ __global__ __launch_bounds__(kFewThreads) void few_rows_kernel(const Product a) 
 #pragma unroll
         for (int i = 0; i < kAhead; ++i) {
             const int64_t k = k0 + i * kFewWaves * kEach + g * Form<T>::kLane;
-            fq[i] = direct(q + k, has_col ? a.k - k : 0);
-            fp[i] = direct(p + k, has_row ? a.k - k : 0);
+            fq[i] = formed<T>(read<T, Form<T>::kLane>(q + k, has_col ? a.k - k : 0));
+            fp[i] = formed<T>(read<T, Form<T>::kLane>(p + k, has_row ? a.k - k : 0));
         }
 #pragma unroll
         for (int i = 0; i < kAhead; ++i) acc = mma(fq[i], fp[i], acc);
@@ -1284,6 +1335,66 @@ __global__ __launch_bounds__(kFewThreads) void few_rows_kernel(const Product a) 
     if (j.slope_out != nullptr) {
         using Slope = typename Form<TO>::Slope;
         static_cast<Slope*>(j.slope_out)[o] = static_cast<Slope>(d[0]);
+    }
+}
+
+// Narrow layers: the weight's fragments stay in registers, and every wavefront takes sixteen
+// rows after sixteen rows through them, straight from memory (a lane's operand of an
+// instruction is 16 or 32 consecutive bytes of a row; the next rows are on their way while
+// these are multiplied).  No barriers, LDS only on the way out.  Bound by memory: 524 288 rows
+// of 64 float32 to 64, of softplus.
+// KS: steps of k (4 kLane values each), KC: times sixteen columns.
+constexpr int kNarrowThreads = 256;
+template <typename T, typename TO, int KS, int KC>
+__global__ __launch_bounds__(kNarrowThreads, 2) void narrow_kernel(const Product a) {
+    using Out = Finish<TO, KC, kLinearForward, Form<T>::kScaled, false>;
+    constexpr int L = Form<T>::kLane;
+    __shared__ __attribute__((aligned(16))) char lds[kNarrowThreads / 64 * Out::kBytes];
+    const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), g = lane >> 4;
+    char* space = lds + wave * Out::kBytes;
+    Fragment<T> fq[KS][KC];
+#pragma unroll
+    for (int c = 0; c < KC; ++c) {
+        const int64_t col = c * 16 + (lane & 15);
+        const bool there = col < a.q.rows;
+        const T* q = static_cast<const T*>(a.q.p) + (there ? col : 0) * a.q.stride;
+#pragma unroll
+        for (int s = 0; s < KS; ++s) {
+            const int64_t k = (s * 4 + g) * L;
+            fq[s][c] = formed<T>(read<T, L>(q + k, there ? a.k - k : 0));
+        }
+    }
+    Out out;
+    out.start(a, 0);
+    const int64_t step = static_cast<int64_t>(gridDim.x) * (kNarrowThreads / 64) * 16;
+    int64_t row0 = (static_cast<int64_t>(blockIdx.x) * (kNarrowThreads / 64) + wave) * 16;
+    Values<T, L> next[KS];
+    const auto load = [&](int64_t first) {
+        const int64_t row = first + (lane & 15);
+        const bool there = row < a.p.rows;
+        const T* p = static_cast<const T*>(a.p.p) + (there ? row : 0) * a.p.stride;
+#pragma unroll
+        for (int s = 0; s < KS; ++s) {
+            const int64_t k = (s * 4 + g) * L;
+            next[s] = read<T, L>(p + k, there ? a.k - k : 0);
+        }
+    };
+    if (row0 < a.p.rows) load(row0);
+    for (; row0 < a.p.rows; row0 += step) {
+        f32x4 acc[KC];
+#pragma unroll
+        for (int c = 0; c < KC; ++c) acc[c] = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
+        Fragment<T> fp[KS];
+#pragma unroll
+        for (int s = 0; s < KS; ++s) fp[s] = formed<T>(next[s]);
+        if (row0 + step < a.p.rows) load(row0 + step);
+#pragma unroll
+        for (int s = 0; s < KS; ++s) {
+#pragma unroll
+            for (int c = 0; c < KC; ++c) acc[c] = mma(fq[s][c], fp[s], acc[c]);
+        }
+        out.give(space, acc);
+        out.rows(a, space, row0);
     }
 }
 
@@ -1323,6 +1434,11 @@ __global__ __launch_bounds__(kJoinThreads) void join_kernel(const float* parts, 
 constexpr int64_t kFewRows = 64;
 
 int64_t tiles_of(int64_t n, int size) { return (n + size - 1) / size; }
+int power_of(int64_t n) {   // the next power of two, up to 64
+    int p = 1;
+    while (p < n && p < 64) p *= 2;
+    return p;
+}
 
 template <typename T, typename TO, int BR, int BC, int KIND>
 int launch(Product a, hipStream_t s) {
@@ -1355,6 +1471,34 @@ int launch_large(Product a, hipStream_t s) {
     return 0;
 }
 
+// Registers of a weight's fragments, in 16 bytes a lane; up to 32 fit beside the rows' own
+// (8-bit rows, which are wider or have to be formed, leave less).
+template <typename T> constexpr int narrow_registers(int ks, int kc) {
+    return ks * kc * Form<T>::kParts * (Form<T>::kIsByte ? 2 : 1);
+}
+template <typename T> constexpr bool narrow_fits(int ks, int kc) {
+    return narrow_registers<T>(ks, kc) <= 32 && (!Form<T>::kScaled || ks * kc < 16 || (ks < 4 && Form<T>::kIsByte));
+}
+
+template <typename T, typename TO, int KS, int KC> int launch_narrow(const Product& a, hipStream_t s) {
+    if constexpr (narrow_fits<T>(KS, KC)) {
+        const int64_t groups = tiles_of(a.p.rows, kNarrowThreads / 64 * 16);
+        // as many workgroups as are under way at once
+        const int64_t most = narrow_registers<T>(KS, KC) <= 12 ? 1024 : 512;
+        narrow_kernel<T, TO, KS, KC><<<static_cast<unsigned>(groups < most ? groups : most), kNarrowThreads, 0, s>>>(a);
+        ASH_LAUNCH_CHECK();
+    }
+    return 0;
+}
+template <typename T, typename TO, int KS> int launch_narrow(const Product& a, int kc, hipStream_t s) {
+    switch (kc) {
+        case 1: return launch_narrow<T, TO, KS, 1>(a, s);
+        case 2: return launch_narrow<T, TO, KS, 2>(a, s);
+        case 4: return launch_narrow<T, TO, KS, 4>(a, s);
+        default: return launch_narrow<T, TO, KS, 8>(a, s);
+    }
+}
+
 template <typename T, typename TO, int KIND>
 int launch_by_size(const Product& a, hipStream_t s) {
     if constexpr (KIND == kLinearForward) {
@@ -1364,6 +1508,14 @@ int launch_by_size(const Product& a, hipStream_t s) {
                                      kFewThreads, 0, s>>>(a);
             ASH_LAUNCH_CHECK();
             return 0;
+        }
+    }
+    if constexpr (KIND == kLinearForward) {
+        const int ks = power_of(tiles_of(a.k, 4 * Form<T>::kLane)), kc = power_of(tiles_of(a.q.rows, 16));
+        if (ks <= 4 && kc <= 8 && narrow_fits<T>(ks, kc)) {
+            if (ks == 1) return launch_narrow<T, TO, 1>(a, kc, s);
+            if (ks == 2) return launch_narrow<T, TO, 2>(a, kc, s);
+            return launch_narrow<T, TO, 4>(a, kc, s);
         }
     }
     if constexpr (KIND == kLinearGradWeight) {
@@ -1428,14 +1580,14 @@ int linear_run<ASH_LINEAR_DTYPE>(LinearKind kind, const LinearJob& j, hipStream_
                 a.other_stride = j.second_stride;
                 return launch_by_size<T, T, kLinearSecond>(a, s);
             case kLinearGradInput:
-                a.p = {j.grad, j.slope, j.cols, j.rows, j.slope_factor};
+                a.p = {j.grad, j.slope, j.cols, j.rows, j.slope_factor, j.slope_kind};
                 a.q = {j.weight, nullptr, j.in, j.in, 1.0f};
                 a.k = j.cols;
                 return launch_by_size<T, T, kLinearGradInput>(a, s);
             case kLinearGradWeight: {
-                a.p = {j.grad, j.slope, j.cols, j.cols, j.slope_factor};
+                a.p = {j.grad, j.slope, j.cols, j.cols, j.slope_factor, j.slope_kind};
                 a.q = {j.input, nullptr, j.input_stride, j.in, 1.0f};
-                a.p2 = {j.second_grad, j.second_slope, j.cols, j.cols, j.slope_factor};
+                a.p2 = {j.second_grad, j.second_slope, j.cols, j.cols, j.slope_factor, j.slope_kind};
                 a.q2 = {j.second_factor, nullptr, j.second_stride, j.in, 1.0f};
                 a.k = j.rows;
                 a.pairs = j.second_grad != nullptr ? 2 : 1;
