@@ -997,6 +997,16 @@ int ash_linear_backward_weight(const ash_linear_args* args, const void* grad, co
                                const void* second_input, int64_t second_input_stride,
                                int second_has_bias, void* grad_weight, void* grad_bias,
                                void* scratch, int64_t scratch_bytes, void* stream);
+/* Both gradients in one pass over the rows, for up to 64 features in and out (and at
+ * least one row): scratch_bytes is 0 where the two calls above have to be made.  With a
+ * second pair grad_input and grad_bias are those of that pair. */
+int64_t ash_linear_backward_both_scratch_bytes(int64_t rows, int64_t in_features,
+                                               int64_t out_features, int32_t dtype, int pairs);
+int ash_linear_backward_both(const ash_linear_args* args, const void* grad, const void* slope,
+                             const void* second_grad, const void* second_slope,
+                             const void* second_input, int64_t second_input_stride,
+                             void* grad_input, void* grad_weight, void* grad_bias,
+                             void* scratch, int64_t scratch_bytes, void* stream);
 /* Second order.  second_input (or NULL) is the gradient of grad_input, addend (or
  * NULL) what the gradients of grad_weight (V) and grad_bias (c) give: input V^T + c.  With t = second_input weight^T + addend:
  *   grad_grad = t f'(z),  curvature = t grad f''(z)   (either NULL)

@@ -28,7 +28,8 @@ def leaves(*tensors):
 
 # one row to several tiles, every tail of a chunk, a step and a tile
 SHAPES = [(1, 1, 1), (1, 64, 64), (5, 3, 2), (16, 131, 33), (17, 8, 31), (64, 256, 100), (65, 19, 64), (127, 64, 1),
-          (130, 67, 129), (300, 200, 257), (1000, 33, 65), (2049, 64, 64), (4100, 19, 128)]
+          (130, 67, 129), (300, 200, 257), (1000, 33, 65), (2049, 64, 64), (4100, 19, 128), (777, 40, 24),
+          (513, 24, 50), (40000, 31, 30)]
 ACTS = [("none", 1.0), ("relu", 1.0), ("silu", 1.0), ("gelu", 1.0), ("softplus", 100.0), ("sine", 30.0)]
 
 
@@ -88,7 +89,7 @@ def test_activations(gpu_ash, kind, a, dtype):
 
 @pytest.mark.parametrize("dtype", TYPES, ids=ids)
 @pytest.mark.parametrize("kind,a", ACTS)
-@pytest.mark.parametrize("shape", [(3, 5, 4), (200, 67, 129), (1030, 64, 64)], ids=str)
+@pytest.mark.parametrize("shape", [(3, 5, 4), (200, 67, 129), (1030, 64, 64), (700, 20, 50), (40000, 50, 20)], ids=str)
 def test_second_order(gpu_ash, shape, kind, a, dtype):
     x, w, b, _, gy, u = operands(*shape, dtype, seed=1, a=a, sine=kind == "sine")
     _, d, dd, _ = ref.linear(x, w, b, kind, a)

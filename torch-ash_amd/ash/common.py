@@ -392,6 +392,12 @@ _SIGNATURES = {
         ctypes.c_int,
         [ctypes.POINTER(_LinearArgs)] + [_PTR] * 5 + [_I64, ctypes.c_int] + [_PTR] * 3 + [_I64, _PTR],
     ),
+    "ash_linear_backward_both_scratch_bytes": (
+        _I64, [_I64, _I64, _I64, ctypes.c_int32, ctypes.c_int]
+    ),
+    "ash_linear_backward_both": (
+        ctypes.c_int, [ctypes.POINTER(_LinearArgs)] + [_PTR] * 5 + [_I64] + [_PTR] * 4 + [_I64, _PTR],
+    ),
     "ash_linear_second": (
         ctypes.c_int,
         [ctypes.POINTER(_LinearArgs), _PTR, _PTR, _I64, _PTR, _I64, _PTR, _PTR, _PTR],

@@ -17,6 +17,7 @@
 
 #include <dlfcn.h>
 
+#include <array>
 #include <memory>
 #include <mutex>
 #include <optional>
@@ -78,6 +79,8 @@ namespace py = pybind11;
     X(ash_linear_scale_gradient)                                                      \
     X(ash_linear_backward_weight_scratch_bytes)                                       \
     X(ash_linear_backward_weight)                                                     \
+    X(ash_linear_backward_both_scratch_bytes)                                         \
+    X(ash_linear_backward_both)                                                       \
     X(ash_linear_second)                                                              \
     X(ash_norm_forward)                                                               \
     X(ash_norm_backward_scratch_bytes)                                                \
@@ -1134,6 +1137,27 @@ std::pair<Tensor, Tensor> linear_backward_weight(const Pair& one, const Pair& tw
     return {gw, gb};
 }
 
+// All gradients at once, of (input, weight, bias); nothing where the layer is not narrow.
+// Of two pairs the input's and the bias' gradients are those of the second.
+std::optional<std::array<Tensor, 3>> linear_backward_both(const Pair& one, const Pair& two, const Tensor& w,
+                                                          bool need_bias, const Activation& f) {
+    const Tensor& grad = one.grad;
+    const int64_t device = grad.get_device();
+    const bool pairs = two.grad.defined();
+    ash_linear_args a = linear_args(one.input, w, Tensor(), f);
+    const int64_t bytes = lib.ash_linear_backward_both_scratch_bytes(a.rows, a.in_features, a.out_features, a.dtype,
+                                                                     pairs ? 2 : 1);
+    if (bytes == 0) return std::nullopt;
+    const Tensor gx = empty({a.rows, a.in_features}, grad.scalar_type(), device);
+    const Tensor gw = empty({a.out_features, a.in_features}, grad.scalar_type(), device);
+    const Tensor gb = need_bias ? empty({a.out_features}, grad.scalar_type(), device) : Tensor();
+    const Tensor scratch = empty({bytes}, at::kByte, device);
+    check(lib.ash_linear_backward_both(&a, grad.data_ptr(), ptr<void>(one.slope), ptr<void>(two.grad),
+                                       ptr<void>(two.slope), ptr<void>(two.input), stride_of(two.input), gx.data_ptr(),
+                                       gw.data_ptr(), ptr<void>(gb), scratch.data_ptr(), bytes, stream_of(device)));
+    return std::array<Tensor, 3>{gx, gw, gb};
+}
+
 // A backward pass that is captured into a graph while an eager graph of the same leaves
 // lives would hand their gradients to nodes of the default stream, which may not wait for
 // a stream that is being captured: the process ends there.  Refused here, where an error
@@ -1167,6 +1191,12 @@ struct LinearGrad : torch::autograd::Function<LinearGrad> {
         ctx->saved_data["needs"] = (need_x ? 1 : 0) | (need_w ? 2 : 0) | (need_b ? 4 : 0);
         ctx->set_materialize_grads(false);
         variable_list out;
+        if (need_x && need_w) {
+            if (const auto all = linear_backward_both({grad, d, x}, {}, w, need_b, f)) {
+                for (int i = 0; i < (need_b ? 3 : 2); ++i) out.push_back((*all)[i]);
+                return out;
+            }
+        }
         if (need_x) out.push_back(linear_backward_input(grad, d, w, Tensor(), f));
         if (need_w || need_b) {
             auto [gw, gb] = linear_backward_weight({grad, d, x}, {}, false, need_w, need_b, f);
@@ -1209,6 +1239,12 @@ struct LinearGrad : torch::autograd::Function<LinearGrad> {
                                         stride_of(addend), ptr<void>(of_grad), ptr<void>(q), stream_of(device)));
         }
         out[0] = of_grad;
+        if (need_x && need_w && u.defined() && q.defined() && !of_w.defined()) {
+            if (const auto all = linear_backward_both({grad, d, u}, {q, Tensor(), x}, w, need_b, f)) {
+                for (int i = 0; i < 3; ++i) out[i + 1] = (*all)[i];
+                return out;
+            }
+        }
         if (need_x) {
             if (of_w.defined()) out[1] = linear_backward_input(grad, d, of_w, Tensor(), f);
             if (q.defined()) out[1] = linear_backward_input(q, Tensor(), w, out[1], f);
@@ -1270,7 +1306,13 @@ struct Linear : torch::autograd::Function<Linear> {
         Tensor grad = grads[0].contiguous(), d = slope;
         const Activation f{static_cast<int32_t>(ctx->saved_data["kind"].toInt()), ctx->saved_data["scale"].toDouble(),
                            by_output};
-        if (need_x && need_w) scale_gradient(grad, d, x, w, f);
+        if (need_x && need_w) {
+            if (const auto all = linear_backward_both({grad, d, readable(x)}, {}, w.contiguous(), need_b, f)) {
+                for (int i = 0; i < 3; ++i) out[i] = (*all)[i];
+                return out;
+            }
+            scale_gradient(grad, d, x, w, f);
+        }
         if (need_x) out[0] = linear_backward_input(grad, d, w.contiguous(), Tensor(), f);
         if (need_w || need_b) {
             std::tie(out[1], out[2]) = linear_backward_weight({grad, d, readable(x)}, {}, false, need_w, need_b, f);

@@ -664,13 +664,52 @@ int ash_linear_backward_weight(const ash_linear_args* args, const void* grad, co
     j.second_factor = second_input;
     j.second_stride = second_input_stride;
     j.second_has_bias = second_has_bias != 0;
-    j.out = grad_weight;
+    j.weight_out = grad_weight;
     j.bias_out = grad_bias;
     j.scratch = scratch;
     j.splits = args->rows > 0 ? linear_splits(args->rows, args->in_features, args->out_features, args->dtype, pairs) : 1;
     PointerGuard guard;
     ASH_HIP(guard.enter_for(grad_weight != nullptr ? grad_weight : grad_bias));
     return run_linear(kLinearGradWeight, j, args->dtype, static_cast<hipStream_t>(stream));
+}
+
+int64_t ash_linear_backward_both_scratch_bytes(int64_t rows, int64_t in_features, int64_t out_features, int32_t dtype,
+                                               int pairs) {
+    if (rows <= 0 || in_features < 1 || out_features < 1 || in_features > kNarrowFeatures ||
+        out_features > kNarrowFeatures || pairs < 1 || (dtype != ASH_F32 && dtype != ASH_BF16 && dtype != ASH_F16)) {
+        return 0;
+    }
+    return narrow_backward_parts(rows, pairs) * (in_features * out_features + out_features) * 4;
+}
+
+int ash_linear_backward_both(const ash_linear_args* args, const void* grad, const void* slope, const void* second_grad,
+                             const void* second_slope, const void* second_input, int64_t second_input_stride,
+                             void* grad_input, void* grad_weight, void* grad_bias, void* scratch, int64_t scratch_bytes,
+                             void* stream) {
+    if (check_linear(args, false, "linear_backward_both") != 0) return 1;
+    const int pairs = second_grad != nullptr ? 2 : 1;
+    const int64_t bytes = ash_linear_backward_both_scratch_bytes(args->rows, args->in_features, args->out_features,
+                                                                 args->dtype, pairs);
+    if (bytes == 0) ASH_FAIL("linear_backward_both takes rows of up to 64 features in and out");
+    if (grad == nullptr || grad_input == nullptr || grad_weight == nullptr || scratch == nullptr ||
+        (pairs == 2 && second_input == nullptr) || second_input_stride < 0) {
+        ASH_FAIL("null pointer in linear_backward_both");
+    }
+    if (scratch_bytes < bytes) ASH_FAIL("linear_backward_both: the scratch is too small");
+    LinearJob j = job_of(*args);
+    j.grad = grad;
+    j.slope = slope;
+    j.second_grad = second_grad;
+    j.second_slope = second_slope;
+    j.second_factor = second_input;
+    j.second_stride = second_input_stride;
+    j.out = grad_input;
+    j.weight_out = grad_weight;
+    j.bias_out = grad_bias;
+    j.scratch = scratch;
+    PointerGuard guard;
+    ASH_HIP(guard.enter_for(grad));
+    return run_linear(kLinearGradBoth, j, args->dtype, static_cast<hipStream_t>(stream));
 }
 
 int ash_linear_second(const ash_linear_args* args, const void* grad, const void* second_input,

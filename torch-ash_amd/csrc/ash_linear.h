@@ -42,12 +42,13 @@ struct LinearJob {
     const void* second_factor;
     int64_t second_stride;
     bool second_has_bias;     // which pair's grad the bias' gradient sums
+    void* weight_out;         // of the weight's gradient (`out`: the input's)
     void* bias_out;
     void* scratch;
     int32_t splits;           // parts the rows are cut into, per pair
 };
 
-enum LinearKind { kLinearForward, kLinearGradInput, kLinearGradWeight, kLinearSecond };
+enum LinearKind { kLinearForward, kLinearGradInput, kLinearGradWeight, kLinearSecond, kLinearGradBoth };
 
 // Defined in ash_linear.hip, one set for every type.
 template <int DTYPE>
@@ -63,6 +64,14 @@ inline WeightTile weight_tile(int64_t in, int64_t out, int32_t dtype) {
     if (dtype == ASH_F32 || in <= 64) return {128, 64};
     if (in > 512 && out > 512) return {256, 256};
     return {128, 128};
+}
+
+// Gradients of input and weight in one kernel: layers of up to 64 features in and out.
+constexpr int64_t kNarrowFeatures = 64;
+// Its workgroups (two a CU), each of which leaves a part of the weight's gradient.
+inline int64_t narrow_backward_parts(int64_t rows, int pairs) {
+    const int64_t slabs = (rows + 63) / 64 * pairs;
+    return slabs < 512 ? slabs : 512;
 }
 
 // Parts that the rows are cut into for a weight's gradient (ash_layers.hip).

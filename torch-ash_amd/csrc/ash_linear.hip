@@ -1398,6 +1398,196 @@ __global__ __launch_bounds__(kNarrowThreads, 2) void narrow_kernel(const Product
     }
 }
 
+// The gradients of a narrow layer (up to 64 features in and out) in one pass over the rows:
+// 64 rows at a time, gz = grad * slope and the input, formed once, lie in LDS as rows of
+// features, which the input's gradient reads along (a wavefront has sixteen rows of it) and
+// the weight's reads turned (a wavefront has sixteen of its rows, or some columns of them).
+// The next rows are on their way into registers meanwhile.  Persistent workgroups; each
+// leaves a part of the weight's gradient, which join_kernel joins.
+//
+// A second pair of operands (second order) is gone through after the first; the input's
+// gradient and the bias' are of the last pair.
+constexpr int kSlab = 64;   // rows at a time
+
+// Byte of 16-byte piece `c` of row `n` of rows of RB bytes, such that neither eight or sixteen
+// rows read along nor four and four rows read turned meet a bank twice.
+template <int RB> __device__ inline int both_place(int n, int c) {
+    if constexpr (RB == 128) return n * 128 + ((c ^ ((n & 2) | ((n >> 1) & 4) | ((n >> 2) & 1))) << 4);
+    else return n * 64 + ((c ^ ((n >> 2) & 3)) << 4);
+}
+
+template <typename T, int MT, int KT>
+__global__ __launch_bounds__(kNarrowThreads, 2) void narrow_backward_kernel(const Product a) {
+    using Out = Finish<T, KT, kLinearGradInput, false, false>;
+    using F = Form<T>;
+    using M = typename F::Slope;
+    constexpr int kParts = F::kParts, kMB = MT * 32, kKB = KT * 32;   // bytes of a row
+    constexpr int kGz = kSlab * kMB, kX = kSlab * kKB, kW = KT * 16 * kMB;
+    constexpr int kPlanes = kParts * (kGz + kX), kSpace = 4 * Out::kBytes;
+    constexpr bool kApart = sizeof(T) == 2;   // the way out has LDS of its own (float32: there would be one workgroup a CU)
+    constexpr int kOperands = kApart || kPlanes > kSpace ? kPlanes : kSpace;
+    constexpr int kEachM = MT / 2, kEachK = KT / 2;                   // units of eight values a thread
+    constexpr int kWaveM = MT < 4 ? MT : 4, kWaveK = 4 / kWaveM, kC = KT / kWaveK;
+    __shared__ __attribute__((aligned(16))) char lds[kOperands + kParts * kW + (kApart ? kSpace : 0)];
+    char* const gz = lds;
+    char* const x = lds + kParts * kGz;
+    char* const wt = lds + kOperands;
+    const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), g = lane >> 4;
+    char* const space = (kApart ? wt + kParts * kW : lds) + wave * Out::kBytes;
+    const int64_t rows = a.k, out_features = a.job.cols, in_features = a.q.rows;
+
+    const auto put8 = [&](char* plane, int part_bytes, int at, const float (&v)[8]) {
+        if constexpr (kParts == 3) {
+            const Three t = split(v);
+#pragma unroll
+            for (int part = 0; part < 3; ++part) __builtin_memcpy(plane + part * part_bytes + at, &t.part[part], 16);
+        } else {
+            *reinterpret_cast<uint4*>(plane + at) = packed<T>(v);
+        }
+    };
+    // the weight, turned: row k, along m
+    const bool wants_input = a.job.out != nullptr;
+    if (wants_input) {
+        for (int u = threadIdx.x; u < KT * 16 * MT * 2; u += kNarrowThreads) {
+            const int k = u % (KT * 16), c = u / (KT * 16);
+            float v[8];
+#pragma unroll
+            for (int i = 0; i < 8; ++i) {
+                const int m = c * 8 + i;
+                v[i] = m < out_features && k < in_features
+                               ? as_float(static_cast<const T*>(a.job.weight)[m * in_features + k]) : 0.0f;
+            }
+            put8(wt, kW, both_place<kMB>(k, c), v);
+        }
+    }
+
+    Values<T, 8> vg[kEachM], vx[kEachK];
+    Values<M, 8> vd[kEachM];
+    const int64_t slabs = (rows + kSlab - 1) / kSlab, all = slabs * a.pairs;
+    const auto load = [&](int64_t slab) {
+        const bool second = slab >= slabs;
+        const Side& p = second ? a.p2 : a.p;
+        const Side& q = second ? a.q2 : a.q;
+        const int64_t row0 = (second ? slab - slabs : slab) * kSlab;
+#pragma unroll
+        for (int i = 0; i < kEachM; ++i) {
+            const int u = threadIdx.x + i * kNarrowThreads;
+            const int64_t row = row0 + u / (MT * 2), m = u % (MT * 2) * 8;
+            const int64_t left = row < rows ? out_features - m : 0;
+            vg[i] = read<T, 8>(static_cast<const T*>(p.p) + row * p.stride + m, left);
+            if (p.mul != nullptr) vd[i] = read<M, 8>(static_cast<const M*>(p.mul) + row * p.stride + m, left);
+        }
+#pragma unroll
+        for (int i = 0; i < kEachK; ++i) {
+            const int u = threadIdx.x + i * kNarrowThreads;
+            const int64_t row = row0 + u / (KT * 2), k = u % (KT * 2) * 8;
+            vx[i] = read<T, 8>(static_cast<const T*>(q.p) + row * q.stride + k, row < rows ? in_features - k : 0);
+        }
+    };
+    // sixteen rows' values along a row's piece, or sixteen columns' values down rows
+    const auto along = [&](const char* plane, auto row_bytes, int part_bytes, int row0, int inner) {
+        Fragment<T> f;
+#pragma unroll
+        for (int part = 0; part < kParts; ++part) {
+            const char* at = plane + part * part_bytes + both_place<decltype(row_bytes)::value>(row0 + (lane & 15), inner * 4 + g);
+            if constexpr (kParts == 3) __builtin_memcpy(&f.v[part], at, 16);
+            else __builtin_memcpy(&f.v, at, 16);
+        }
+        return f;
+    };
+    const auto down = [&](char* plane, auto row_bytes, int part_bytes, int col0, int inner) {
+        Fragment<T> f;
+        const int i = lane & 15, n = inner * 32 + g * 8 + (i >> 2), col = col0 + (i & 3) * 4;
+#pragma unroll
+        for (int part = 0; part < kParts; ++part) {
+            i16x4 half[2];
+#pragma unroll
+            for (int h = 0; h < 2; ++h) {
+                char* at = plane + part * part_bytes + both_place<decltype(row_bytes)::value>(n + h * 4, col >> 3) + (col & 7) * 2;
+                half[h] = __builtin_amdgcn_ds_read_tr16_b64_v4i16((__attribute__((address_space(3))) i16x4*)at);
+            }
+            if constexpr (kParts == 3) __builtin_memcpy(&f.v[part], half, 16);
+            else __builtin_memcpy(&f.v, half, 16);
+        }
+        return f;
+    };
+    using RowM = std::integral_constant<int, kMB>;
+    using RowK = std::integral_constant<int, kKB>;
+    const int tile_m = wave % kWaveM, tile_k = wave / kWaveM * kC;
+    const bool has_bias = a.job.bias_out != nullptr && tile_k == 0;
+
+    Out out;
+    out.start(a, 0);
+    f32x4 acc[kC], bias_sum = {0.0f, 0.0f, 0.0f, 0.0f};
+#pragma unroll
+    for (int c = 0; c < kC; ++c) acc[c] = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
+    if (blockIdx.x < all) load(blockIdx.x);
+    for (int64_t slab = blockIdx.x; slab < all; slab += gridDim.x) {
+        const bool last = slab >= slabs * (a.pairs - 1), second = slab >= slabs;
+        const Side& p = second ? a.p2 : a.p;
+        __syncthreads();   // of the last slab's reads
+#pragma unroll
+        for (int i = 0; i < kEachM; ++i) {
+            const int u = threadIdx.x + i * kNarrowThreads;
+            float v[8];
+#pragma unroll
+            for (int e = 0; e < 8; ++e) v[e] = as_float(vg[i].v[e]);
+            if (p.mul != nullptr) {
+#pragma unroll
+                for (int e = 0; e < 8; ++e) v[e] *= slope_of<T>(as_float(vd[i].v[e]), p.kind, p.factor);
+            }
+            put8(gz, kGz, both_place<kMB>(u / (MT * 2), u % (MT * 2)), v);
+        }
+#pragma unroll
+        for (int i = 0; i < kEachK; ++i) {
+            const int u = threadIdx.x + i * kNarrowThreads;
+            float v[8];
+#pragma unroll
+            for (int e = 0; e < 8; ++e) v[e] = as_float(vx[i].v[e]);
+            put8(x, kX, both_place<kKB>(u / (KT * 2), u % (KT * 2)), v);
+        }
+        __syncthreads();
+        if (slab + gridDim.x < all) load(slab + gridDim.x);
+        f32x4 of_input[KT];
+        const bool input = wants_input && last;
+        if (input) {
+#pragma unroll
+            for (int c = 0; c < KT; ++c) of_input[c] = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
+#pragma unroll
+            for (int inner = 0; inner < MT / 2; ++inner) {
+                const Fragment<T> fp = along(gz, RowM{}, kGz, wave * 16, inner);
+#pragma unroll
+                for (int c = 0; c < KT; ++c) of_input[c] = mma(along(wt, RowM{}, kW, c * 16, inner), fp, of_input[c]);
+            }
+        }
+#pragma unroll
+        for (int inner = 0; inner < kSlab / 32; ++inner) {
+            const Fragment<T> fp = down(gz, RowM{}, kGz, tile_m * 16, inner);
+#pragma unroll
+            for (int c = 0; c < kC; ++c) acc[c] = mma(down(x, RowK{}, kX, (tile_k + c) * 16, inner), fp, acc[c]);
+            if (has_bias && last) bias_sum = sum_rows(fp, bias_sum);
+        }
+        if (input) {
+            if constexpr (!kApart) __syncthreads();   // of this slab's reads: the way out goes over them
+            out.give(space, of_input);
+            out.rows(a, space, (second ? slab - slabs : slab) * kSlab + wave * 16);
+        }
+    }
+    float* part = static_cast<float*>(a.job.scratch) + blockIdx.x * (out_features * in_features + out_features);
+    const int64_t m = tile_m * 16 + (lane & 15);
+    if (m < out_features) {
+#pragma unroll
+        for (int c = 0; c < kC; ++c) {
+            const int64_t k = (tile_k + c) * 16 + g * 4;
+#pragma unroll
+            for (int i = 0; i < 4; ++i) {
+                if (k + i < in_features) part[m * in_features + k + i] = acc[c][i];
+            }
+        }
+        if (has_bias && g == 0) part[out_features * in_features + m] = bias_sum[0];
+    }
+}
+
 // Joins the parts of a weight's gradient, in their order.
 constexpr int kJoinThreads = 256, kJoin = 32;   // values a workgroup, eight threads each
 template <typename T>
@@ -1499,6 +1689,26 @@ template <typename T, typename TO, int KS> int launch_narrow(const Product& a, i
     }
 }
 
+template <typename T> int join(const LinearJob& j, int64_t parts, int64_t bias_first, int64_t bias_parts, hipStream_t s) {
+    const int64_t values = j.cols * j.in, groups = tiles_of(values + j.cols, kJoin);
+    join_kernel<T><<<static_cast<unsigned>(groups), kJoinThreads, 0, s>>>(
+            static_cast<const float*>(j.scratch), values, j.cols, parts, bias_first, bias_parts,
+            static_cast<T*>(j.weight_out), static_cast<T*>(j.bias_out));
+    ASH_LAUNCH_CHECK();
+    return 0;
+}
+
+template <typename T> int launch_narrow_backward(const Product& a, hipStream_t s) {
+    const unsigned grid = static_cast<unsigned>(narrow_backward_parts(a.k, a.pairs));
+    const bool m = a.job.cols > 32, k = a.q.rows > 32;
+    if (m && k) narrow_backward_kernel<T, 4, 4><<<grid, kNarrowThreads, 0, s>>>(a);
+    else if (m) narrow_backward_kernel<T, 4, 2><<<grid, kNarrowThreads, 0, s>>>(a);
+    else if (k) narrow_backward_kernel<T, 2, 4><<<grid, kNarrowThreads, 0, s>>>(a);
+    else narrow_backward_kernel<T, 2, 2><<<grid, kNarrowThreads, 0, s>>>(a);
+    ASH_LAUNCH_CHECK();
+    return 0;
+}
+
 template <typename T, typename TO, int KIND>
 int launch_by_size(const Product& a, hipStream_t s) {
     if constexpr (KIND == kLinearForward) {
@@ -1596,14 +1806,22 @@ int linear_run<ASH_LINEAR_DTYPE>(LinearKind kind, const LinearJob& j, hipStream_
                 const int64_t steps = tiles_of(j.rows, Form<T>::kStep);
                 a.part_rows = tiles_of(steps, j.splits) * Form<T>::kStep;
                 if (j.rows > 0 && launch_by_size<T, T, kLinearGradWeight>(a, s) != 0) return 1;
-                const int64_t values = j.cols * j.in, parts = j.rows > 0 ? a.parts * a.pairs : 0;
-                const int64_t groups = tiles_of(values + j.cols, kJoin);
-                join_kernel<T><<<static_cast<unsigned>(groups), kJoinThreads, 0, s>>>(
-                        static_cast<const float*>(j.scratch), values, j.cols, parts,
-                        a.second_has_bias ? a.parts : 0, j.rows > 0 ? a.parts : 0, static_cast<T*>(j.out),
-                        static_cast<T*>(j.bias_out));
-                ASH_LAUNCH_CHECK();
-                return 0;
+                return join<T>(j, j.rows > 0 ? a.parts * a.pairs : 0, a.second_has_bias ? a.parts : 0,
+                               j.rows > 0 ? a.parts : 0, s);
+            }
+            case kLinearGradBoth: {
+                a.p = {j.grad, j.slope, j.cols, j.rows, j.slope_factor, j.slope_kind};
+                a.q = {j.input, nullptr, j.input_stride, j.in, 1.0f};
+                a.p2 = {j.second_grad, j.second_slope, j.cols, j.rows, j.slope_factor, j.slope_kind};
+                a.q2 = {j.second_factor, nullptr, j.second_stride, j.in, 1.0f};
+                a.k = j.rows;
+                a.pairs = j.second_grad != nullptr ? 2 : 1;
+                a.job.bias = nullptr;
+                a.job.residual = nullptr;
+                a.job.slope_out = nullptr;
+                a.job.activation = ASH_ACT_NONE;
+                if (launch_narrow_backward<T>(a, s) != 0) return 1;
+                return join<T>(j, narrow_backward_parts(j.rows, a.pairs), 0, narrow_backward_parts(j.rows, a.pairs), s);
             }
             default:
                 break;
