@@ -1345,55 +1345,95 @@ __global__ __launch_bounds__(kFewThreads) void few_rows_kernel(const Product a) 
 // of 64 float32 to 64, of softplus.
 // KS: steps of k (4 kLane values each), KC: times sixteen columns.
 constexpr int kNarrowThreads = 256;
-template <typename T, typename TO, int KS, int KC>
+template <typename T, typename TO, int KS, int KC, int KIND>
 __global__ __launch_bounds__(kNarrowThreads, 2) void narrow_kernel(const Product a) {
-    using Out = Finish<TO, KC, kLinearForward, Form<T>::kScaled, false>;
+    using Out = Finish<TO, KC, KIND, Form<T>::kScaled, false>;
+    using M = typename Form<T>::Slope;
     constexpr int L = Form<T>::kLane;
-    __shared__ __attribute__((aligned(16))) char lds[kNarrowThreads / 64 * Out::kBytes];
+    constexpr bool kGrad = KIND == kLinearGradInput, kTwo = KIND == kLinearSecond;
+    constexpr int kSpace = Out::kBytes * (kTwo ? 2 : 1);
+    __shared__ __attribute__((aligned(16))) char lds[kNarrowThreads / 64 * kSpace];
     const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), g = lane >> 4;
-    char* space = lds + wave * Out::kBytes;
+    char* space = lds + wave * kSpace;
     Fragment<T> fq[KS][KC];
 #pragma unroll
     for (int c = 0; c < KC; ++c) {
         const int64_t col = c * 16 + (lane & 15);
         const bool there = col < a.q.rows;
-        const T* q = static_cast<const T*>(a.q.p) + (there ? col : 0) * a.q.stride;
+        const T* q = static_cast<const T*>(a.q.p) + (there ? col : 0) * (kGrad ? 1 : a.q.stride);
 #pragma unroll
         for (int s = 0; s < KS; ++s) {
-            const int64_t k = (s * 4 + g) * L;
-            fq[s][c] = formed<T>(read<T, L>(q + k, there ? a.k - k : 0));
+            const int64_t k = (s * 4 + g) * L, left = there ? a.k - k : 0;
+            if constexpr (kGrad) {   // the weight lies across
+                Values<T, L> v;
+                __builtin_memset(&v, 0, sizeof(v));
+#pragma unroll
+                for (int i = 0; i < L; ++i) {
+                    if (i < left) v.v[i] = q[(k + i) * a.q.stride];
+                }
+                fq[s][c] = formed<T>(v);
+            } else {
+                fq[s][c] = formed<T>(read<T, L>(q + k, left));
+            }
         }
     }
     Out out;
     out.start(a, 0);
     const int64_t step = static_cast<int64_t>(gridDim.x) * (kNarrowThreads / 64) * 16;
     int64_t row0 = (static_cast<int64_t>(blockIdx.x) * (kNarrowThreads / 64) + wave) * 16;
-    Values<T, L> next[KS];
+    Values<T, L> next[KS], other[kTwo ? KS : 1];
+    Values<M, L> slope[kGrad ? KS : 1];
+    const bool mul = kGrad && a.p.mul != nullptr;
     const auto load = [&](int64_t first) {
         const int64_t row = first + (lane & 15);
         const bool there = row < a.p.rows;
-        const T* p = static_cast<const T*>(a.p.p) + (there ? row : 0) * a.p.stride;
+        const int64_t at = there ? row : 0;
 #pragma unroll
         for (int s = 0; s < KS; ++s) {
-            const int64_t k = (s * 4 + g) * L;
-            next[s] = read<T, L>(p + k, there ? a.k - k : 0);
+            const int64_t k = (s * 4 + g) * L, left = there ? a.k - k : 0;
+            next[s] = read<T, L>(static_cast<const T*>(a.p.p) + at * a.p.stride + k, left);
+            if constexpr (kTwo) {
+                other[s] = read<T, L>(static_cast<const T*>(a.other) + at * a.other_stride + k, a.other != nullptr ? left : 0);
+            }
+            if constexpr (kGrad) {
+                if (mul) slope[s] = read<M, L>(static_cast<const M*>(a.p.mul) + at * a.p.stride + k, left);
+            }
         }
     };
     if (row0 < a.p.rows) load(row0);
     for (; row0 < a.p.rows; row0 += step) {
-        f32x4 acc[KC];
+        f32x4 acc[KC], more[kTwo ? KC : 1];
+        Fragment<T> fp[KS], fo[kTwo ? KS : 1];
 #pragma unroll
-        for (int c = 0; c < KC; ++c) acc[c] = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
-        Fragment<T> fp[KS];
+        for (int s = 0; s < KS; ++s) {
+            if constexpr (kGrad) {
+                if (mul) {
 #pragma unroll
-        for (int s = 0; s < KS; ++s) fp[s] = formed<T>(next[s]);
+                    for (int i = 0; i < L; ++i) {
+                        next[s].v[i] = static_cast<T>(as_float(next[s].v[i]) *
+                                                      slope_of<T>(as_float(slope[s].v[i]), a.p.kind, a.p.factor));
+                    }
+                }
+            }
+            fp[s] = formed<T>(next[s]);
+            if constexpr (kTwo) fo[s] = formed<T>(other[s]);
+        }
         if (row0 + step < a.p.rows) load(row0 + step);
+#pragma unroll
+        for (int c = 0; c < KC; ++c) {
+            acc[c] = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
+            if constexpr (kTwo) more[c] = acc[c];
+        }
 #pragma unroll
         for (int s = 0; s < KS; ++s) {
 #pragma unroll
-            for (int c = 0; c < KC; ++c) acc[c] = mma(fq[s][c], fp[s], acc[c]);
+            for (int c = 0; c < KC; ++c) {
+                acc[c] = mma(fq[s][c], fp[s], acc[c]);
+                if constexpr (kTwo) more[c] = mma(fq[s][c], fo[s], more[c]);
+            }
         }
         out.give(space, acc);
+        if constexpr (kTwo) out.give(space, more, 1);
         out.rows(a, space, row0);
     }
 }
@@ -1662,30 +1702,31 @@ int launch_large(Product a, hipStream_t s) {
 }
 
 // Registers of a weight's fragments, in 16 bytes a lane; up to 32 fit beside the rows' own
-// (8-bit rows, which are wider or have to be formed, leave less).
+// (8-bit rows, which are wider or have to be formed, leave less, and so do gradients, whose
+// rows come in twos).
 template <typename T> constexpr int narrow_registers(int ks, int kc) {
     return ks * kc * Form<T>::kParts * (Form<T>::kIsByte ? 2 : 1);
 }
-template <typename T> constexpr bool narrow_fits(int ks, int kc) {
-    return narrow_registers<T>(ks, kc) <= 32 && (!Form<T>::kScaled || ks * kc < 16 || (ks < 4 && Form<T>::kIsByte));
+template <typename T> constexpr bool narrow_fits(int kind, int ks, int kc) {
+    return narrow_registers<T>(ks, kc) <= (kind != kLinearForward && ks == 4 ? 16 : 32) && (!Form<T>::kScaled || ks * kc < 16 || (ks < 4 && Form<T>::kIsByte));
 }
 
-template <typename T, typename TO, int KS, int KC> int launch_narrow(const Product& a, hipStream_t s) {
-    if constexpr (narrow_fits<T>(KS, KC)) {
+template <typename T, typename TO, int KIND, int KS, int KC> int launch_narrow(const Product& a, hipStream_t s) {
+    if constexpr (narrow_fits<T>(KIND, KS, KC)) {
         const int64_t groups = tiles_of(a.p.rows, kNarrowThreads / 64 * 16);
         // as many workgroups as are under way at once
-        const int64_t most = narrow_registers<T>(KS, KC) <= 12 ? 1024 : 512;
-        narrow_kernel<T, TO, KS, KC><<<static_cast<unsigned>(groups < most ? groups : most), kNarrowThreads, 0, s>>>(a);
+        const int64_t most = KIND != kLinearSecond && narrow_registers<T>(KS, KC) <= 12 ? 1024 : 512;
+        narrow_kernel<T, TO, KS, KC, KIND><<<static_cast<unsigned>(groups < most ? groups : most), kNarrowThreads, 0, s>>>(a);
         ASH_LAUNCH_CHECK();
     }
     return 0;
 }
-template <typename T, typename TO, int KS> int launch_narrow(const Product& a, int kc, hipStream_t s) {
+template <typename T, typename TO, int KIND, int KS> int launch_narrow(const Product& a, int kc, hipStream_t s) {
     switch (kc) {
-        case 1: return launch_narrow<T, TO, KS, 1>(a, s);
-        case 2: return launch_narrow<T, TO, KS, 2>(a, s);
-        case 4: return launch_narrow<T, TO, KS, 4>(a, s);
-        default: return launch_narrow<T, TO, KS, 8>(a, s);
+        case 1: return launch_narrow<T, TO, KIND, KS, 1>(a, s);
+        case 2: return launch_narrow<T, TO, KIND, KS, 2>(a, s);
+        case 4: return launch_narrow<T, TO, KIND, KS, 4>(a, s);
+        default: return launch_narrow<T, TO, KIND, KS, 8>(a, s);
     }
 }
 
@@ -1720,12 +1761,12 @@ int launch_by_size(const Product& a, hipStream_t s) {
             return 0;
         }
     }
-    if constexpr (KIND == kLinearForward) {
+    if constexpr (KIND != kLinearGradWeight) {
         const int ks = power_of(tiles_of(a.k, 4 * Form<T>::kLane)), kc = power_of(tiles_of(a.q.rows, 16));
-        if (ks <= 4 && kc <= 8 && narrow_fits<T>(ks, kc)) {
-            if (ks == 1) return launch_narrow<T, TO, 1>(a, kc, s);
-            if (ks == 2) return launch_narrow<T, TO, 2>(a, kc, s);
-            return launch_narrow<T, TO, 4>(a, kc, s);
+        if (ks <= 4 && kc <= 8 && narrow_fits<T>(KIND, ks, kc)) {
+            if (ks == 1) return launch_narrow<T, TO, KIND, 1>(a, kc, s);
+            if (ks == 2) return launch_narrow<T, TO, KIND, 2>(a, kc, s);
+            return launch_narrow<T, TO, KIND, 4>(a, kc, s);
         }
     }
     if constexpr (KIND == kLinearGradWeight) {
