@@ -154,10 +154,12 @@ template <typename T> __device__ inline uint4 packed(const float (&v)[8]) {
     return u;
 }
 
-// exp(x) by the unit's exp2: the argument's product with log2(e) in two parts, of which the
-// second, below a step of the first, is applied as a factor.
-__device__ inline float exp_of(float x) {
+// exp(x) by the unit's exp2.  FULL: the argument's product with log2(e) in two parts, of which
+// the second, below a step of the first, is applied as a factor; without, the error is 2^-24
+// of the argument, which results of 16 bits do not show.
+template <bool FULL> __device__ inline float exp_of(float x) {
     const float t = x * 1.44269504f;
+    if constexpr (!FULL) return __builtin_amdgcn_exp2f(t);
     const float rest = fmaf(x, 1.44269504f, -t) + x * 1.92596299e-8f;
     const float e = __builtin_amdgcn_exp2f(t);
     // (beyond the range of float the first part says all there is)
@@ -174,7 +176,7 @@ template <typename T> __device__ inline float slope_of(float kept, int kind, flo
         if (kind == kSlopeSoftplus) {
             const float t = factor * kept;   // (the factor is a)
             const float near = t * fmaf(t, fmaf(t, fmaf(t, -0.041666668f, 0.16666667f), -0.5f), 1.0f);
-            return t < 0.03125f ? near : 1.0f - exp_of(-t);
+            return t < 0.03125f ? near : 1.0f - exp_of<true>(-t);
         }
     }
     return factor * kept;
@@ -482,12 +484,12 @@ __device__ inline f32x4 sum_rows(const Fragment<float>& p, f32x4 c) {
 }
 
 // --------------------------------------------------------------------- activations
-__device__ inline float sigmoid(float v) { return __builtin_amdgcn_rcpf(1.0f + exp_of(-v)); }
+template <bool FULL> __device__ inline float sigmoid(float v) { return __builtin_amdgcn_rcpf(1.0f + exp_of<FULL>(-v)); }
 
 // The normal distribution's integral and its density at z.  The complementary error function
 // is t exp(-x^2 + P(t)), t = 1 / (1 + x / 2), with the Chebyshev fit erfcc of Press et al.,
 // Numerical Recipes (1.2e-7 of the value, everywhere).
-__device__ inline void normal(float z, float& integral, float& density) {
+template <bool FULL> __device__ inline void normal(float z, float& integral, float& density) {
     const float x = fabsf(z) * 0.70710678f, t = __builtin_amdgcn_rcpf(fmaf(0.5f, x, 1.0f));
     float p = 0.17087277f;
     p = fmaf(p, t, -0.82215223f);
@@ -499,7 +501,7 @@ __device__ inline void normal(float z, float& integral, float& density) {
     p = fmaf(p, t, 0.37409196f);
     p = fmaf(p, t, 1.00002368f);
     p = fmaf(p, t, -1.26551223f);
-    const float e = exp_of(-0.5f * z * z), tail = 0.5f * t * e * exp_of(p);
+    const float e = exp_of<FULL>(-0.5f * z * z), tail = 0.5f * t * e * exp_of<FULL>(p);
     integral = z > 0.0f ? 1.0f - tail : tail;
     density = 0.39894228f * e;
 }
@@ -538,7 +540,7 @@ __device__ inline void sine_cosine(float x, float& sine, float& cosine) {
 // of them to the operands' type would be one more of the size of that of gz and of the
 // result (half as much again in the gradients' error).  That of a sine is kept without the
 // factor a, so that all fit fp16 (they are at most 1.13).
-template <int N>
+template <bool FULL, int N>
 __device__ inline void activate(int kind, float a, const float (&z)[N], float (&y)[N], float (&d)[N]) {
     switch (kind) {
         case ASH_ACT_RELU:
@@ -551,7 +553,7 @@ __device__ inline void activate(int kind, float a, const float (&z)[N], float (&
         case ASH_ACT_SILU:
 #pragma unroll
             for (int i = 0; i < N; ++i) {
-                const float p = sigmoid(z[i]);
+                const float p = sigmoid<FULL>(z[i]);
                 y[i] = z[i] * p;
                 d[i] = p * fmaf(z[i], 1.0f - p, 1.0f);
             }
@@ -560,7 +562,7 @@ __device__ inline void activate(int kind, float a, const float (&z)[N], float (&
 #pragma unroll
             for (int i = 0; i < N; ++i) {
                 float c, density;
-                normal(z[i], c, density);
+                normal<FULL>(z[i], c, density);
                 y[i] = z[i] * c;
                 d[i] = fmaf(z[i], density, c);
             }
@@ -569,7 +571,7 @@ __device__ inline void activate(int kind, float a, const float (&z)[N], float (&
             const float inverse = 1.0f / a;
 #pragma unroll
             for (int i = 0; i < N; ++i) {
-                const float v = a * z[i], e = exp_of(-fabsf(v)), r = __builtin_amdgcn_rcpf(1.0f + e);
+                const float v = a * z[i], e = exp_of<FULL>(-fabsf(v)), r = __builtin_amdgcn_rcpf(1.0f + e);
                 y[i] = fmaf(log_of_one_and(e), inverse, v < 0.0f ? 0.0f : z[i]);
                 d[i] = v < 0.0f ? e * r : r;
             }
@@ -589,13 +591,13 @@ __device__ inline void activate(int kind, float a, const float (&z)[N], float (&
 }
 
 // f'(z) (whole, of a sine too) and f''(z)
-template <int N>
+template <bool FULL, int N>
 __device__ inline void curve(int kind, float a, const float (&z)[N], float (&d)[N], float (&dd)[N]) {
     switch (kind) {
         case ASH_ACT_SILU:
 #pragma unroll
             for (int i = 0; i < N; ++i) {
-                const float p = sigmoid(z[i]);
+                const float p = sigmoid<FULL>(z[i]);
                 d[i] = p * fmaf(z[i], 1.0f - p, 1.0f);
                 dd[i] = p * (1.0f - p) * fmaf(z[i], 1.0f - 2.0f * p, 2.0f);
             }
@@ -604,7 +606,7 @@ __device__ inline void curve(int kind, float a, const float (&z)[N], float (&d)[
 #pragma unroll
             for (int i = 0; i < N; ++i) {
                 float c, density;
-                normal(z[i], c, density);
+                normal<FULL>(z[i], c, density);
                 d[i] = fmaf(z[i], density, c);
                 dd[i] = fmaf(-z[i], z[i], 2.0f) * density;
             }
@@ -612,7 +614,7 @@ __device__ inline void curve(int kind, float a, const float (&z)[N], float (&d)[
         case ASH_ACT_SOFTPLUS:
 #pragma unroll
             for (int i = 0; i < N; ++i) {
-                const float v = a * z[i], e = exp_of(-fabsf(v)), r = __builtin_amdgcn_rcpf(1.0f + e);
+                const float v = a * z[i], e = exp_of<FULL>(-fabsf(v)), r = __builtin_amdgcn_rcpf(1.0f + e);
                 d[i] = v < 0.0f ? e * r : r;
                 dd[i] = a * e * r * r;
             }
@@ -655,18 +657,20 @@ struct Product {
     const void* other;
     int64_t other_stride;
     int64_t row_tiles, col_tiles;
+    bool stream;
     LinearJob job;
 };
 
-// STREAM: past the caches (of the large tiles' outputs, which fill them several times over,
-// 65 536 rows of 1024 bf16: 171 -> 158 us).
-template <typename T, int N, bool STREAM> __device__ inline void put_values(T* out, int64_t left, const float (&v)[N]) {
+// stream: past the caches, for outputs that would fill the L2s (32 MB): 65 536 rows of 1024
+// bf16 171 -> 158 us, 524 288 of 64 float32 77 -> 74, their input's gradient 110 -> 96.
+constexpr int64_t kStreamBytes = 32 << 20;
+template <typename T, int N> __device__ inline void put_values(T* out, int64_t left, const float (&v)[N], bool stream) {
     typedef uint32_t Word __attribute__((ext_vector_type(N * sizeof(T) / 4), aligned(2)));
     Values<T, N> r;
 #pragma unroll
     for (int i = 0; i < N; ++i) r.v[i] = static_cast<T>(v[i]);
     if (left >= N) {
-        if constexpr (STREAM) {
+        if (stream) {
             Word w;
             __builtin_memcpy(&w, &r, sizeof(r));
             __builtin_nontemporal_store(w, reinterpret_cast<Word*>(out));
@@ -730,7 +734,7 @@ template <typename T, int BR, int BC> struct Shared {
 // waits for another.  (Straight from the registers, where a lane has four columns of a row, or
 // sixteen if the columns are dealt out for that, lines go in pieces: 524 288 rows of 64
 // float32, with slopes, 200 us for 145 by way of LDS.)
-template <typename TO, int KC, int KIND, bool SCALED, bool STREAM>
+template <typename TO, int KC, int KIND, bool SCALED>
 struct Finish {
     using Slope = typename Form<TO>::Slope;
     static constexpr bool kTwo = KIND == kLinearSecond;
@@ -769,65 +773,75 @@ struct Finish {
             __builtin_memcpy(v + 4 * h, from + (r * kPieces + piece) * 16, 16);
         }
     }
+    // first_row: the same for a wavefront, so that a row's address is a scalar one and the
+    // lane's offset from it
     __device__ void rows(const Product& a, const char* space, int64_t first_row) const {
         const LinearJob& j = a.job;
+        const int r0 = lane / kLanes;
+        const int32_t offset = r0 * static_cast<int32_t>(a.q.rows) + static_cast<int32_t>(col);
+        const int64_t rows_left = a.p.rows - first_row;
 #pragma unroll 1
-        for (int r = lane / kLanes; r < 16; r += kDown) {
-            const int64_t row = first_row + r;
-            if (row >= a.p.rows || left <= 0) continue;
+        for (int i = 0; i < 16 / kDown + (16 % kDown != 0); ++i) {
+            const int r = r0 + i * kDown;
+            if (r >= 16 || r >= rows_left || left <= 0) continue;
+            const int64_t row = first_row + i * kDown, o = row * a.q.rows;   // (of lane 0)
             float z[N], y[N], d[N];
             take(space, r, z);
-            const float row_scale = SCALED ? j.input_scales[row] : 1.0f;
+            const float row_scale = SCALED ? j.input_scales[row + r0] : 1.0f;
 #pragma unroll
-            for (int i = 0; i < N; ++i) {
-                if constexpr (SCALED) z[i] *= row_scale * scale[i];
-                z[i] += bias[i];
+            for (int e = 0; e < N; ++e) {
+                if constexpr (SCALED) z[e] *= row_scale * scale[e];
+                z[e] += bias[e];
             }
-            const int64_t o = row * a.q.rows + col;
             if constexpr (kTwo) {
                 // t: the derivative of <second input, gradient of the input> by gz
                 float t[N], g[N], dd[N];
                 take(space + kBytes, r, t);
                 if (j.addend != nullptr) {
-                    get_values(static_cast<const TO*>(j.addend) + row * j.addend_stride + col, left, g);
+                    get_values(static_cast<const TO*>(j.addend) + row * j.addend_stride + (r0 * j.addend_stride + col), left, g);
 #pragma unroll
-                    for (int i = 0; i < N; ++i) t[i] += g[i];
+                    for (int e = 0; e < N; ++e) t[e] += g[e];
                 }
-                get_values(static_cast<const TO*>(j.grad) + o, left, g);
-                curve(j.activation, j.act_scale, z, d, dd);
+                get_values(static_cast<const TO*>(j.grad) + o + offset, left, g);
+                curve<sizeof(TO) == 4>(j.activation, j.act_scale, z, d, dd);
 #pragma unroll
-                for (int i = 0; i < N; ++i) {
-                    y[i] = t[i] * d[i];
-                    dd[i] *= t[i] * g[i];
+                for (int e = 0; e < N; ++e) {
+                    y[e] = t[e] * d[e];
+                    dd[e] *= t[e] * g[e];
                 }
-                if (j.out != nullptr) put_values<TO, N, STREAM>(static_cast<TO*>(j.out) + o, left, y);
-                if (j.curvature_out != nullptr) put_values<TO, N, STREAM>(static_cast<TO*>(j.curvature_out) + o, left, dd);
+                if (j.out != nullptr) put_values(static_cast<TO*>(j.out) + o + offset, left, y, a.stream);
+                if (j.curvature_out != nullptr) {
+                    put_values(static_cast<TO*>(j.curvature_out) + o + offset, left, dd, a.stream);
+                }
             } else {
                 float more[N];
                 if (j.residual != nullptr) {
-                    get_values(static_cast<const TO*>(j.residual) + row * j.residual_stride + col, left, more);
+                    get_values(static_cast<const TO*>(j.residual) + row * j.residual_stride + (r0 * j.residual_stride + col),
+                               left, more);
                 }
-                activate(j.activation, j.act_scale, z, y, d);
+                activate<sizeof(TO) == 4>(j.activation, j.act_scale, z, y, d);
+                if (j.slope_out != nullptr) {
+                    put_values(static_cast<Slope*>(j.slope_out) + o + offset, left, d, a.stream);
+                }
                 if (j.residual != nullptr) {
 #pragma unroll
-                    for (int i = 0; i < N; ++i) y[i] += more[i];
+                    for (int e = 0; e < N; ++e) y[e] += more[e];
                 }
-                put_values<TO, N, STREAM>(static_cast<TO*>(j.out) + o, left, y);
-                if (j.slope_out != nullptr) put_values<Slope, N, STREAM>(static_cast<Slope*>(j.slope_out) + o, left, d);
+                put_values(static_cast<TO*>(j.out) + o + offset, left, y, a.stream);
             }
         }
     }
 };
 
 // The same of all of a wavefront's rows of a tile.
-template <typename TO, int BR, int BC, int KIND, bool SCALED, bool STREAM>
+template <typename TO, int BR, int BC, int KIND, bool SCALED>
 __device__ inline void finish(const Product& a, char* space, const f32x4 (&acc)[Tile<BR, BC>::kR][Tile<BR, BC>::kC],
                               int64_t row0, int64_t col0) {
     using W = Tile<BR, BC>;
     constexpr bool kTwo = KIND == kLinearSecond;
     constexpr int kTiles = kTwo ? W::kR / 2 : W::kR;
     const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
-    Finish<TO, W::kC, KIND, SCALED, STREAM> out;
+    Finish<TO, W::kC, KIND, SCALED> out;
     out.start(a, col0 + wave % W::kWaveCols * W::kC * 16);
     const int64_t first_row = row0 + wave / W::kWaveCols * kTiles * 16;
 #pragma unroll 1
@@ -992,7 +1006,7 @@ __global__ __launch_bounds__((Tile<BR, BC>::kThreads)) void product_kernel(const
         leave_part<BR, BC>(a, acc, rows_sum, w.part, row0, col0, w.sums);
     } else {
         __syncthreads();   // of all wavefronts' reads of their operands
-        finish<TO, BR, BC, KIND, Form<T>::kScaled, false>(a, lds + wave * W::kOutBytes * (KIND == kLinearSecond ? 2 : 1), acc,
+        finish<TO, BR, BC, KIND, Form<T>::kScaled>(a, lds + wave * W::kOutBytes * (KIND == kLinearSecond ? 2 : 1), acc,
                                                    row0, col0);
     }
 }
@@ -1268,7 +1282,7 @@ __global__ __launch_bounds__(kLargeThreads) void large_kernel(const Product a) {
         work.template run<false>({p0, q0}, {p1, q1}, {p2, q2}, {p3, q3});
         __syncthreads();   // of all wavefronts' reads of their operands
         char* space = (work.wave < 4 ? p0 : q0) + work.wave % 4 * LargeTile::kOutBytes;
-        finish<TO, kLarge, kLarge, KIND, Form<T>::kScaled, true>(a, space, work.acc, row0, col0);
+        finish<TO, kLarge, kLarge, KIND, Form<T>::kScaled>(a, space, work.acc, row0, col0);
     }
 }
 
@@ -1328,7 +1342,7 @@ __global__ __launch_bounds__(kFewThreads) void few_rows_kernel(const Product a) 
     const LinearJob& j = a.job;
     if constexpr (Form<T>::kScaled) z[0] *= j.input_scales[out_row] * j.weight_scales[out_col];
     if (j.bias != nullptr) z[0] += as_float(static_cast<const TO*>(j.bias)[out_col]);
-    activate(j.activation, j.act_scale, z, y, d);
+    activate<sizeof(TO) == 4>(j.activation, j.act_scale, z, y, d);
     if (j.residual != nullptr) y[0] += as_float(static_cast<const TO*>(j.residual)[out_row * j.residual_stride + out_col]);
     const int64_t o = out_row * a.q.rows + out_col;
     static_cast<TO*>(j.out)[o] = static_cast<TO>(y[0]);
@@ -1347,7 +1361,7 @@ __global__ __launch_bounds__(kFewThreads) void few_rows_kernel(const Product a) 
 constexpr int kNarrowThreads = 256;
 template <typename T, typename TO, int KS, int KC, int KIND>
 __global__ __launch_bounds__(kNarrowThreads, 2) void narrow_kernel(const Product a) {
-    using Out = Finish<TO, KC, KIND, Form<T>::kScaled, false>;
+    using Out = Finish<TO, KC, KIND, Form<T>::kScaled>;
     using M = typename Form<T>::Slope;
     constexpr int L = Form<T>::kLane;
     constexpr bool kGrad = KIND == kLinearGradInput, kTwo = KIND == kLinearSecond;
@@ -1458,7 +1472,7 @@ template <int RB> __device__ inline int both_place(int n, int c) {
 
 template <typename T, int MT, int KT>
 __global__ __launch_bounds__(kNarrowThreads, 2) void narrow_backward_kernel(const Product a) {
-    using Out = Finish<T, KT, kLinearGradInput, false, false>;
+    using Out = Finish<T, KT, kLinearGradInput, false>;
     using F = Form<T>;
     using M = typename F::Slope;
     constexpr int kParts = F::kParts, kMB = MT * 32, kKB = KT * 32;   // bytes of a row
@@ -1628,35 +1642,48 @@ __global__ __launch_bounds__(kNarrowThreads, 2) void narrow_backward_kernel(cons
     }
 }
 
-// Joins the parts of a weight's gradient, in their order.
-constexpr int kJoinThreads = 256, kJoin = 32;   // values a workgroup, eight threads each
-template <typename T>
+// Joins the parts of a weight's gradient, in their order: kJoin values a workgroup, four a
+// thread, whose other threads share out the parts.
+constexpr int kJoinThreads = 256;
+template <typename T, int kJoin>
 __global__ __launch_bounds__(kJoinThreads) void join_kernel(const float* parts, int64_t values, int64_t bias_values,
-                                                        int64_t n_parts, int64_t bias_first, int64_t bias_parts,
-                                                        T* weight, T* bias) {
-    __shared__ float sums[kJoinThreads / kJoin][kJoin];
-    const int64_t at = static_cast<int64_t>(blockIdx.x) * kJoin + threadIdx.x % kJoin;
-    const int group = threadIdx.x / kJoin;
-    constexpr int kGroups = kJoinThreads / kJoin;
-    const int64_t stride = values + bias_values;
-    const bool of_bias = at >= values;
-    const int64_t first = of_bias ? bias_first : 0, n = of_bias ? bias_parts : n_parts;
-    float sum = 0.0f;
-    if (at < stride && (of_bias ? bias != nullptr : weight != nullptr)) {
+                                                            int64_t n_parts, int64_t bias_first, int64_t bias_parts,
+                                                            T* weight, T* bias) {
+    constexpr int kGroups = kJoinThreads / (kJoin / 4);
+    __shared__ f32x4 sums[kGroups][kJoin / 4];
+    const int group = threadIdx.x / (kJoin / 4), lane = threadIdx.x % (kJoin / 4);
+    const int64_t at = static_cast<int64_t>(blockIdx.x) * kJoin + lane * 4;
+    const int64_t stride = values + bias_values, left = values - at;
+    f32x4 sum = {0.0f, 0.0f, 0.0f, 0.0f};
+    const auto add = [&](int64_t first, int64_t n, int64_t from, int64_t most) {
         const int64_t each = (n + kGroups - 1) / kGroups;
-        const int64_t from = first + group * each, to = group * each + each < n ? from + each : first + n;
-#pragma unroll 8
-        for (int64_t part = from; part < to; ++part) sum += parts[part * stride + at];
-    }
-    sums[group][threadIdx.x % kJoin] = sum;
-    __syncthreads();
-    if (group != 0 || at >= stride) return;
+        const int64_t end = (group + 1) * each < n ? (group + 1) * each : n;
+#pragma unroll 4
+        for (int64_t part = group * each; part < end; ++part) {
+            const Values<float, 4> v = read<float, 4>(parts + (first + part) * stride + from, most);
 #pragma unroll
-    for (int i = 1; i < kGroups; ++i) sum += sums[i][threadIdx.x % kJoin];
+            for (int i = 0; i < 4; ++i) sum[i] += v.v[i];
+        }
+    };
+    // workgroups past the weight's values have the bias'
+    const int64_t weight_groups = (values + kJoin - 1) / kJoin;
+    const bool of_bias = static_cast<int64_t>(blockIdx.x) >= weight_groups;
+    const int64_t bias_at = at - weight_groups * kJoin;
     if (of_bias) {
-        if (bias != nullptr) bias[at - values] = static_cast<T>(sum);
+        if (bias != nullptr) add(bias_first, bias_parts, values + bias_at, bias_values - bias_at);
     } else if (weight != nullptr) {
-        weight[at] = static_cast<T>(sum);
+        add(0, n_parts, at, left);
+    }
+    sums[group][lane] = sum;
+    __syncthreads();
+    if (group != 0) return;
+#pragma unroll
+    for (int i = 1; i < kGroups; ++i) sum += sums[i][lane];
+    const float out[4] = {sum[0], sum[1], sum[2], sum[3]};
+    if (of_bias) {
+        if (bias != nullptr && bias_at < bias_values) put_values(bias + bias_at, bias_values - bias_at, out, false);
+    } else if (weight != nullptr && left > 0) {
+        put_values(weight + at, left, out, false);
     }
 }
 
@@ -1731,10 +1758,15 @@ template <typename T, typename TO, int KIND, int KS> int launch_narrow(const Pro
 }
 
 template <typename T> int join(const LinearJob& j, int64_t parts, int64_t bias_first, int64_t bias_parts, hipStream_t s) {
-    const int64_t values = j.cols * j.in, groups = tiles_of(values + j.cols, kJoin);
-    join_kernel<T><<<static_cast<unsigned>(groups), kJoinThreads, 0, s>>>(
-            static_cast<const float*>(j.scratch), values, j.cols, parts, bias_first, bias_parts,
-            static_cast<T*>(j.weight_out), static_cast<T*>(j.bias_out));
+    const int64_t values = j.cols * j.in;
+#define ASH_JOIN(n)                                                                                              \
+    join_kernel<T, n><<<static_cast<unsigned>(tiles_of(values, n) + tiles_of(j.cols, n)), kJoinThreads, 0, s>>>( \
+            static_cast<const float*>(j.scratch), values, j.cols, parts, bias_first, bias_parts,                 \
+            static_cast<T*>(j.weight_out), static_cast<T*>(j.bias_out))
+    // 32 threads for a value's parts where there are many (narrow layers), or eight
+    if (parts > 64) ASH_JOIN(32);
+    else ASH_JOIN(128);
+#undef ASH_JOIN
     ASH_LAUNCH_CHECK();
     return 0;
 }
@@ -1806,6 +1838,8 @@ int linear_run<ASH_LINEAR_DTYPE>(LinearKind kind, const LinearJob& j, hipStream_
     using T = Operand;
     Product a{};
     a.job = j;
+    a.stream = j.rows * (kind == kLinearForward || kind == kLinearSecond ? j.cols : j.in) *
+                       (j.out_dtype == ASH_F32 ? 4 : 2) >= kStreamBytes;
     switch (kind) {
         case kLinearForward:
             a.p = {j.input, nullptr, j.input_stride, j.rows, 1.0f};
