@@ -52,7 +52,8 @@ def test_linear_and_its_gradients(gpu_ash, shape, dtype):
 
 @pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16], ids=ids)
 @pytest.mark.parametrize("rows,k,m,kind", [(16640, 1032, 1000, "gelu"), (20001, 520, 776, "none"),
-                                           (33000, 256, 512, "sine"), (4100, 2056, 544, "silu")])
+                                           (33000, 256, 512, "sine"), (4100, 2056, 544, "silu"),
+                                           (10007, 136, 264, "softplus"), (2500, 1032, 1000, "relu"), (3333, 80, 104, "none")])
 def test_linear_and_its_gradients_in_large_tiles(gpu_ash, rows, k, m, kind, dtype):
     """Sizes that end inside a tile and inside a step, an odd number of steps; aligned
     and not (the other tiles take those)."""
@@ -278,7 +279,8 @@ def test_rows_beyond_32_bits(gpu_ash):
 # --------------------------------------------------------------------- 8-bit rows
 @pytest.mark.parametrize("out_dtype", TYPES, ids=ids)
 @pytest.mark.parametrize("shape", [(1, 16, 1), (1, 1024, 64), (7, 3, 5), (16, 131, 33), (40, 600, 48), (65, 128, 64),
-                                   (130, 67, 129), (1000, 257, 300), (16500, 400, 1008)], ids=str)
+                                   (130, 67, 129), (1000, 257, 300), (16500, 400, 1008), (2500, 272, 1000),
+                                   (9000, 2064, 136)], ids=str)
 def test_linear_of_8_bit_rows(gpu_ash, shape, out_dtype):
     rows, k, m = shape
     x, w, b, r, _, _ = operands(rows, k, m, torch.float32, seed=11)

@@ -780,8 +780,10 @@ struct Finish {
         const int r0 = lane / kLanes;
         const int32_t offset = r0 * static_cast<int32_t>(a.q.rows) + static_cast<int32_t>(col);
         const int64_t rows_left = a.p.rows - first_row;
-#pragma unroll 1
-        for (int i = 0; i < 16 / kDown + (16 % kDown != 0); ++i) {
+        // (where there is nothing to compute, all at once: gradients of 524 288 rows of 64 float32
+        // 132 -> 120 us)
+#pragma unroll KIND == kLinearGradInput ? 4 : 1
+        for (int i = 0; i < (16 + kDown - 1) / kDown; ++i) {
             const int r = r0 + i * kDown;
             if (r >= 16 || r >= rows_left || left <= 0) continue;
             const int64_t row = first_row + i * kDown, o = row * a.q.rows;   // (of lane 0)
@@ -819,9 +821,14 @@ struct Finish {
                     get_values(static_cast<const TO*>(j.residual) + row * j.residual_stride + (r0 * j.residual_stride + col),
                                left, more);
                 }
-                activate<sizeof(TO) == 4>(j.activation, j.act_scale, z, y, d);
-                if (j.slope_out != nullptr) {
-                    put_values(static_cast<Slope*>(j.slope_out) + o + offset, left, d, a.stream);
+                if constexpr (KIND == kLinearGradInput) {
+#pragma unroll
+                    for (int e = 0; e < N; ++e) y[e] = z[e];
+                } else {
+                    activate<sizeof(TO) == 4>(j.activation, j.act_scale, z, y, d);
+                    if (j.slope_out != nullptr) {
+                        put_values(static_cast<Slope*>(j.slope_out) + o + offset, left, d, a.stream);
+                    }
                 }
                 if (j.residual != nullptr) {
 #pragma unroll
@@ -1011,24 +1018,25 @@ __global__ __launch_bounds__((Tile<BR, BC>::kThreads)) void product_kernel(const
     }
 }
 
-// Large products of operands of one or two bytes: tiles of 256 x 256, whose operands go from
-// memory into LDS without passing through registers, so that a wavefront can hold 128 x 64
-// sums (with 64 x 64 a wavefront the reads from LDS take as long as the products).  The
+// Products of operands of one or two bytes whose pieces of 16 bytes are aligned: operands go
+// from memory into LDS without passing through registers.  Of tiles of 256 x 256 a wavefront
+// holds 128 x 64 sums (with 64 x 64 the reads from LDS take as long as the products).  The
 // 16-byte pieces of a stage are fetched such that they land where Reader looks for them.
 // Pieces past an operand's end, and past the last k, are outside of the buffer that the
 // loads are told of, and come as zeros.
 //
 // bf16, fp16: four stages of 32 values of k, of which three are on their way while one is
 // multiplied; e4m3, whose instructions take 128 values of k, two.
-constexpr int kLarge = 256, kLargeThreads = 512;
 constexpr uint32_t kNowhere = 0x80000000u;   // beyond every such buffer
 
-template <typename T> struct Stage {
+// SIZE: rows and columns of a tile, 256 or (where those would be too few) 128.
+template <typename T, int SIZE> struct Stage {
+    using W = Tile<SIZE, SIZE>;
     static constexpr int kRow = Form<T>::kIsByte ? 128 : 64;        // bytes of k
     static constexpr int kK = kRow / static_cast<int>(sizeof(T));   // values of k
     static constexpr int kStages = Form<T>::kIsByte ? 2 : 4;
-    static constexpr int kEach = kLarge * kRow / 16 / kLargeThreads;   // pieces a thread and operand
-    static constexpr int kPlane = kLarge * kRow;
+    static constexpr int kEach = SIZE * kRow / 16 / W::kThreads;    // pieces a thread and operand
+    static constexpr int kPlane = SIZE * kRow;
     // stacked: 128 bytes more for every eight rows of k, which puts the rows that a turning
     // read takes together on different banks
     static constexpr int kStacked = kPlane + kK / 8 * 128;
@@ -1039,16 +1047,17 @@ template <typename T> struct Stage {
 };
 constexpr int kWaitAll = 0x0070;
 
-template <typename T, bool STACKED>
+template <typename T, int SIZE, bool STACKED>
 struct Direct {
-    using S = Stage<T>;
+    using S = Stage<T, SIZE>;
+    static constexpr int kThreads = S::W::kThreads;
     const char* base;       // of the tile, at the first k
     uint32_t offset[S::kEach], stride;
     int k_of;               // first k of this thread's pieces along a row
     int64_t extent;         // bytes from base to the operand's end (of k_end)
 
     __device__ void start(const Side& a, int64_t row0, int64_t k0, int64_t k_end) {
-        const int64_t rows = a.rows - row0 < kLarge ? a.rows - row0 : kLarge;
+        const int64_t rows = a.rows - row0 < SIZE ? a.rows - row0 : SIZE;
         stride = static_cast<uint32_t>(a.stride * sizeof(T));
         if constexpr (STACKED) {
             base = static_cast<const char*>(a.p) + (k0 * a.stride + row0) * sizeof(T);
@@ -1060,9 +1069,10 @@ struct Direct {
         k_of = 0;
 #pragma unroll
         for (int i = 0; i < S::kEach; ++i) {
-            const int piece = threadIdx.x + i * kLargeThreads;
+            const int piece = threadIdx.x + i * kThreads;
             if constexpr (STACKED) {
-                const int k = piece >> 5, c = (piece & 31) ^ ((k & 3) << 1);
+                constexpr int kPieces = SIZE / 8;
+                const int k = piece / kPieces, c = piece % kPieces ^ ((k & 3) << 1);
                 offset[i] = k * stride + c * 16;
             } else {
                 constexpr int kPieces = S::kRow / 16;
@@ -1082,9 +1092,10 @@ struct Direct {
         const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
 #pragma unroll
         for (int i = 0; i < S::kEach; ++i) {
-            // a wavefront's pieces are consecutive: stacked, those of two rows of k
-            char* at = plane + wave * 1024 + i * kLargeThreads * 16;
-            if constexpr (STACKED) at += ((wave >> 2) + i * 2) * 128;
+            // a wavefront's pieces are consecutive (stacked: of whole rows of k, of one eight)
+            const int first = wave * 64 + i * kThreads;
+            char* at = plane + first * 16;
+            if constexpr (STACKED) at += first / SIZE * 128;
             __builtin_amdgcn_raw_ptr_buffer_load_lds(
                     buffer, (__attribute__((address_space(3))) void*)at, 16, there ? offset[i] : kNowhere, 0, 0, 0);
         }
@@ -1093,7 +1104,7 @@ struct Direct {
 
 // Where a lane's pieces lie in a stage: addresses differ from one another by constants, or
 // (stacked) go round in four, so that a wavefront keeps a few of them in registers.
-template <typename T, bool STACKED>
+template <typename T, int SIZE, bool STACKED>
 struct Reader {
     static constexpr int kAt = STACKED ? 4 : Form<T>::kIsByte ? 2 : 1;
     const char* at[kAt];
@@ -1104,7 +1115,7 @@ struct Reader {
         for (int n = 0; n < kAt; ++n) {
             if constexpr (STACKED) {
                 const int k = g * 8 + (i >> 2), c = ((row0 >> 3) + ((i & 3) >> 1)) ^ (((k & 3) ^ n) << 1);
-                at[n] = plane + k * kLarge * 2 + g * 128 + (c << 4) + (i & 1) * 8;
+                at[n] = plane + k * SIZE * 2 + g * 128 + (c << 4) + (i & 1) * 8;
             } else if constexpr (Form<T>::kIsByte) {
                 at[n] = plane + (row0 + i) * 128 + (((2 * g + n) ^ (i & 7)) << 4);
             } else {
@@ -1139,7 +1150,7 @@ struct Reader {
                     : "=&v"(part[0]), "=&v"(part[1]), "=&v"(part[2]), "=&v"(part[3]), "=&v"(part[4]), "=&v"(part[5]),
                       "=&v"(part[6]), "=&v"(part[7])
                     : "v"(from[0]), "v"(from[1]), "v"(from[2]), "v"(from[3]), "n"(QUAD * 128),
-                      "n"(QUAD * 128 + 4 * kLarge * 2)
+                      "n"(QUAD * 128 + 4 * SIZE * 2)
                     : "memory");
 #endif
 #pragma unroll
@@ -1162,13 +1173,12 @@ struct Reader {
     }
 };
 
-using LargeTile = Tile<kLarge, kLarge>;
-static_assert(LargeTile::kC == 4 && LargeTile::kR == 8 && LargeTile::kThreads == kLargeThreads, "");
-
-template <typename T, int QUAD, bool SUMS>
+template <typename T, int SIZE, int QUAD, bool SUMS>
 __device__ inline void multiply_quad(const Fragment<T> (&fq)[4], const Fragment<T> (&fp)[4],
-                                     f32x4 (&acc)[LargeTile::kR][4], f32x4 (&rows_sum)[LargeTile::kSums], int wave) {
-    using W = LargeTile;
+                                     f32x4 (&acc)[Tile<SIZE, SIZE>::kR][4], f32x4 (&rows_sum)[Tile<SIZE, SIZE>::kSums],
+                                     int wave) {
+    using W = Tile<SIZE, SIZE>;
+    static_assert(W::kC == 4 && W::kR % 4 == 0, "");
 #pragma unroll
     for (int n = 0; n < 4; ++n) {
         const int r = QUAD * 4 + n;
@@ -1182,13 +1192,13 @@ __device__ inline void multiply_quad(const Fragment<T> (&fq)[4], const Fragment<
 
 // What a wavefront has of a large tile, and what it does in a step.  SUMS: the sums of P's
 // rows too (by the workgroups that are the first of a row of tiles).
-template <typename T, bool STACK_P, bool STACK_Q>
+template <typename T, int SIZE, bool STACK_P, bool STACK_Q>
 struct LargeWork {
-    using W = LargeTile;
-    using S = Stage<T>;
+    using W = Tile<SIZE, SIZE>;
+    using S = Stage<T, SIZE>;
     static constexpr int kP = STACK_P ? S::kStacked : S::kPlane, kQ = STACK_Q ? S::kStacked : S::kPlane;
-    Direct<T, STACK_P> p;
-    Direct<T, STACK_Q> q;
+    Direct<T, SIZE, STACK_P> p;
+    Direct<T, SIZE, STACK_Q> q;
     int length, wave;
     f32x4 acc[W::kR][W::kC], rows_sum[W::kSums];
 
@@ -1222,14 +1232,16 @@ struct LargeWork {
         __builtin_amdgcn_s_barrier();
         asm volatile("" ::: "memory");
         issue(next, k_next);
-        const Reader<T, STACK_P> rp(stage.p, wave / W::kWaveCols * W::kR * 16);
-        const Reader<T, STACK_Q> rq(stage.q, wave % W::kWaveCols * W::kC * 16);
+        const Reader<T, SIZE, STACK_P> rp(stage.p, wave / W::kWaveCols * W::kR * 16);
+        const Reader<T, SIZE, STACK_Q> rq(stage.q, wave % W::kWaveCols * W::kC * 16);
         Fragment<T> fq[4], fp[4];
         rq.template get<0>(fq);
         rp.template get<0>(fp);
-        multiply_quad<T, 0, SUMS>(fq, fp, acc, rows_sum, wave);
-        rp.template get<1>(fp);
-        multiply_quad<T, 1, SUMS>(fq, fp, acc, rows_sum, wave);
+        multiply_quad<T, SIZE, 0, SUMS>(fq, fp, acc, rows_sum, wave);
+        if constexpr (W::kR == 8) {
+            rp.template get<1>(fp);
+            multiply_quad<T, SIZE, 1, SUMS>(fq, fp, acc, rows_sum, wave);
+        }
     }
     // All stages a turn; those past the end are of zeros (a way out between them costs a
     // second set of accumulators).
@@ -1257,12 +1269,14 @@ struct LargeWork {
     }
 };
 
-template <typename T, typename TO, int KIND>
-__global__ __launch_bounds__(kLargeThreads) void large_kernel(const Product a) {
+template <typename T, typename TO, int SIZE, int KIND>
+__global__ __launch_bounds__((Tile<SIZE, SIZE>::kThreads), 2) void large_kernel(const Product a) {
     constexpr bool kStackP = KIND == kLinearGradWeight, kStackQ = KIND != kLinearForward;
-    using Work = LargeWork<T, kStackP, kStackQ>;
-    static_assert(4 * LargeTile::kOutBytes <= Work::kP && 4 * LargeTile::kOutBytes <= Work::kQ, "");
-    constexpr bool kFour = Stage<T>::kStages > 2;
+    using Work = LargeWork<T, SIZE, kStackP, kStackQ>;
+    using W = Tile<SIZE, SIZE>;
+    constexpr int kHalf = W::kWaves / 2;
+    static_assert(kHalf * W::kOutBytes <= Work::kP && kHalf * W::kOutBytes <= Work::kQ, "");
+    constexpr bool kFour = Stage<T, SIZE>::kStages > 2;
     // Planes under names of their own: the compiler then sees that reads of one need not wait
     // for loads into another (it looks only so far through an address, hence one each).
     __shared__ __attribute__((aligned(16))) char p0[Work::kP], p1[Work::kP], p2[kFour ? Work::kP : 16], p3[kFour ? Work::kP : 16];
@@ -1271,18 +1285,18 @@ __global__ __launch_bounds__(kLargeThreads) void large_kernel(const Product a) {
 
     Place w;
     if (!place_of<KIND>(a, w)) return;
-    const int64_t row0 = w.row_tile * kLarge, col0 = w.col_tile * kLarge;
+    const int64_t row0 = w.row_tile * SIZE, col0 = w.col_tile * SIZE;
     Work work;
     work.start(w.second ? a.p2 : a.p, w.second ? a.q2 : a.q, row0, col0, w.k0, w.k_end);
     if constexpr (KIND == kLinearGradWeight) {
         if (w.sums) work.template run<true>({p0, q0}, {p1, q1}, {p2, q2}, {p3, q3});
         else work.template run<false>({p0, q0}, {p1, q1}, {p2, q2}, {p3, q3});
-        leave_part<kLarge, kLarge>(a, work.acc, work.rows_sum, w.part, row0, col0, w.sums);
+        leave_part<SIZE, SIZE>(a, work.acc, work.rows_sum, w.part, row0, col0, w.sums);
     } else {
         work.template run<false>({p0, q0}, {p1, q1}, {p2, q2}, {p3, q3});
         __syncthreads();   // of all wavefronts' reads of their operands
-        char* space = (work.wave < 4 ? p0 : q0) + work.wave % 4 * LargeTile::kOutBytes;
-        finish<TO, kLarge, kLarge, KIND, Form<T>::kScaled>(a, space, work.acc, row0, col0);
+        char* space = (work.wave < kHalf ? p0 : q0) + work.wave % kHalf * W::kOutBytes;
+        finish<TO, SIZE, SIZE, KIND, Form<T>::kScaled>(a, space, work.acc, row0, col0);
     }
 }
 
@@ -1716,14 +1730,14 @@ template <typename T> bool takes_large(const Side& a, int64_t across) {
            across * sizeof(T) % 16 == 0 && a.stride >= across && a.stride < (1 << 21);
 }
 
-template <typename T, typename TO, int KIND>
+template <typename T, typename TO, int SIZE, int KIND>
 int launch_large(Product a, hipStream_t s) {
-    a.row_tiles = tiles_of(a.p.rows, kLarge);
-    a.col_tiles = tiles_of(a.q.rows, kLarge);
+    a.row_tiles = tiles_of(a.p.rows, SIZE);
+    a.col_tiles = tiles_of(a.q.rows, SIZE);
     const int64_t tiles = a.row_tiles * a.col_tiles * (KIND == kLinearGradWeight ? a.parts * a.pairs : 1);
     const int64_t groups = (tiles + kXcds - 1) / kXcds * kXcds;
     if (groups > 0x7FFFFFFFll) ASH_FAIL("linear: too many rows");
-    large_kernel<T, TO, KIND><<<static_cast<unsigned>(groups), kLargeThreads, 0, s>>>(a);
+    large_kernel<T, TO, SIZE, KIND><<<static_cast<unsigned>(groups), Tile<SIZE, SIZE>::kThreads, 0, s>>>(a);
     ASH_LAUNCH_CHECK();
     return 0;
 }
@@ -1806,24 +1820,27 @@ int launch_by_size(const Product& a, hipStream_t s) {
         if (t.cols == 32) return launch<T, TO, 128, 32, KIND>(a, s);
         if (t.rows == 64) return launch<T, TO, 64, 64, KIND>(a, s);
         if constexpr (Form<T>::kParts == 1) {
-            if (t.rows == kLarge && takes_large<T>(a.p, a.p.rows) && takes_large<T>(a.q, a.q.rows) &&
-                (a.pairs == 1 || (takes_large<T>(a.p2, a.p.rows) && takes_large<T>(a.q2, a.q.rows)))) {
-                return launch_large<T, TO, KIND>(a, s);
+            if (t.cols >= 128) {
+                if (takes_large<T>(a.p, a.p.rows) && takes_large<T>(a.q, a.q.rows) &&
+                    (a.pairs == 1 || (takes_large<T>(a.p2, a.p.rows) && takes_large<T>(a.q2, a.q.rows)))) {
+                    return t.cols == 256 ? launch_large<T, TO, 256, KIND>(a, s) : launch_large<T, TO, 128, KIND>(a, s);
+                }
+                return launch<T, TO, 128, 128, KIND>(a, s);
             }
-            if (t.rows == kLarge) return launch<T, TO, 128, 128, KIND>(a, s);
-            if (t.cols == 128) return launch<T, TO, 128, 128, KIND>(a, s);
         }
         return launch<T, TO, 128, 64, KIND>(a, s);
     }
     if (a.q.rows <= 32) return launch<T, TO, 128, 32, KIND>(a, s);
+    if constexpr (Form<T>::kParts == 1 && KIND != kLinearSecond && !std::is_same<T, WideE4M3>::value) {
+        if (a.q.rows > 64 && takes_large<T>(a.p, a.k) && takes_large<T>(a.q, KIND == kLinearForward ? a.k : a.q.rows)) {
+            if (a.q.rows > 128 && tiles_of(a.p.rows, 256) * tiles_of(a.q.rows, 256) >= 256) {
+                return launch_large<T, TO, 256, KIND>(a, s);
+            }
+            if (tiles_of(a.p.rows, 128) * tiles_of(a.q.rows, 128) >= 128) return launch_large<T, TO, 128, KIND>(a, s);
+        }
+    }
     if (tiles_of(a.p.rows, 128) * tiles_of(a.q.rows, 64) < 256) return launch<T, TO, 64, 64, KIND>(a, s);
     if constexpr (Form<T>::kParts == 1) {
-        if constexpr (KIND != kLinearSecond && !std::is_same<T, WideE4M3>::value) {
-            if (a.q.rows > 128 && tiles_of(a.p.rows, kLarge) * tiles_of(a.q.rows, kLarge) >= 256 &&
-                takes_large<T>(a.p, a.k) && takes_large<T>(a.q, KIND == kLinearForward ? a.k : a.q.rows)) {
-                return launch_large<T, TO, KIND>(a, s);
-            }
-        }
         if (a.q.rows > 64) return launch<T, TO, 128, 128, KIND>(a, s);
     }
     return launch<T, TO, 128, 64, KIND>(a, s);
