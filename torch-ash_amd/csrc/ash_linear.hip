@@ -175,8 +175,10 @@ template <typename T> __device__ inline float slope_of(float kept, int kind, flo
         if (kind == kSlopeRelu) return kept > 0.0f ? 1.0f : 0.0f;
         if (kind == kSlopeSoftplus) {
             const float t = factor * kept;   // (the factor is a)
-            const float near = t * fmaf(t, fmaf(t, fmaf(t, -0.041666668f, 0.16666667f), -0.5f), 1.0f);
-            return t < 0.03125f ? near : 1.0f - exp_of<true>(-t);
+            // (the series leaves off 2^-24 of the value at 1/4, the difference 2^-22)
+            const float near = t * fmaf(t, fmaf(t, fmaf(t, fmaf(t, fmaf(t, -1.3888889e-3f, 8.3333333e-3f), -0.041666668f),
+                                                        0.16666667f), -0.5f), 1.0f);
+            return t < 0.25f ? near : 1.0f - exp_of<true>(-t);
         }
     }
     return factor * kept;
@@ -657,26 +659,22 @@ struct Product {
     const void* other;
     int64_t other_stride;
     int64_t row_tiles, col_tiles;
-    bool stream;
     LinearJob job;
 };
 
-// stream: past the caches, for outputs that would fill the L2s (32 MB): 65 536 rows of 1024
-// bf16 171 -> 158 us, 524 288 of 64 float32 77 -> 74, their input's gradient 110 -> 96.
-constexpr int64_t kStreamBytes = 32 << 20;
-template <typename T, int N> __device__ inline void put_values(T* out, int64_t left, const float (&v)[N], bool stream) {
+// Whole pieces go past the caches: what is read of an output next is mostly more than they
+// hold (16 384 rows of 4096 e4m3 to 4096 bf16 316 -> 278 us; of three layers of 64 to 64 in a
+// row one takes 59.7 us for 60.7 of 524 288 rows float32, 10.7 for 11.5 of 131 072 bf16, 27 for
+// 25 of 524 288 bf16, and as long as before of 16 384).
+template <typename T, int N> __device__ inline void put_values(T* out, int64_t left, const float (&v)[N]) {
     typedef uint32_t Word __attribute__((ext_vector_type(N * sizeof(T) / 4), aligned(2)));
     Values<T, N> r;
 #pragma unroll
     for (int i = 0; i < N; ++i) r.v[i] = static_cast<T>(v[i]);
     if (left >= N) {
-        if (stream) {
-            Word w;
-            __builtin_memcpy(&w, &r, sizeof(r));
-            __builtin_nontemporal_store(w, reinterpret_cast<Word*>(out));
-        } else {
-            __builtin_memcpy(out, &r, sizeof(r));
-        }
+        Word w;
+        __builtin_memcpy(&w, &r, sizeof(r));
+        __builtin_nontemporal_store(w, reinterpret_cast<Word*>(out));
     } else {
 #pragma unroll
         for (int i = 0; i < N; ++i) {
@@ -811,9 +809,9 @@ struct Finish {
                     y[e] = t[e] * d[e];
                     dd[e] *= t[e] * g[e];
                 }
-                if (j.out != nullptr) put_values(static_cast<TO*>(j.out) + o + offset, left, y, a.stream);
+                if (j.out != nullptr) put_values(static_cast<TO*>(j.out) + o + offset, left, y);
                 if (j.curvature_out != nullptr) {
-                    put_values(static_cast<TO*>(j.curvature_out) + o + offset, left, dd, a.stream);
+                    put_values(static_cast<TO*>(j.curvature_out) + o + offset, left, dd);
                 }
             } else {
                 float more[N];
@@ -827,14 +825,14 @@ struct Finish {
                 } else {
                     activate<sizeof(TO) == 4>(j.activation, j.act_scale, z, y, d);
                     if (j.slope_out != nullptr) {
-                        put_values(static_cast<Slope*>(j.slope_out) + o + offset, left, d, a.stream);
+                        put_values(static_cast<Slope*>(j.slope_out) + o + offset, left, d);
                     }
                 }
                 if (j.residual != nullptr) {
 #pragma unroll
                     for (int e = 0; e < N; ++e) y[e] += more[e];
                 }
-                put_values(static_cast<TO*>(j.out) + o + offset, left, y, a.stream);
+                put_values(static_cast<TO*>(j.out) + o + offset, left, y);
             }
         }
     }
@@ -1695,9 +1693,9 @@ __global__ __launch_bounds__(kJoinThreads) void join_kernel(const float* parts, 
     for (int i = 1; i < kGroups; ++i) sum += sums[i][lane];
     const float out[4] = {sum[0], sum[1], sum[2], sum[3]};
     if (of_bias) {
-        if (bias != nullptr && bias_at < bias_values) put_values(bias + bias_at, bias_values - bias_at, out, false);
+        if (bias != nullptr && bias_at < bias_values) put_values(bias + bias_at, bias_values - bias_at, out);
     } else if (weight != nullptr && left > 0) {
-        put_values(weight + at, left, out, false);
+        put_values(weight + at, left, out);
     }
 }
 
@@ -1855,8 +1853,6 @@ int linear_run<ASH_LINEAR_DTYPE>(LinearKind kind, const LinearJob& j, hipStream_
     using T = Operand;
     Product a{};
     a.job = j;
-    a.stream = j.rows * (kind == kLinearForward || kind == kLinearSecond ? j.cols : j.in) *
-                       (j.out_dtype == ASH_F32 ? 4 : 2) >= kStreamBytes;
     switch (kind) {
         case kLinearForward:
             a.p = {j.input, nullptr, j.input_stride, j.rows, 1.0f};
