@@ -29,7 +29,7 @@ def leaves(*tensors):
 # one row to several tiles, every tail of a chunk, a step and a tile
 SHAPES = [(1, 1, 1), (1, 64, 64), (5, 3, 2), (16, 131, 33), (17, 8, 31), (64, 256, 100), (65, 19, 64), (127, 64, 1),
           (130, 67, 129), (300, 200, 257), (1000, 33, 65), (2049, 64, 64), (4100, 19, 128), (777, 40, 24),
-          (513, 24, 50), (40000, 31, 30)]
+          (513, 24, 50), (40000, 31, 30), (9000, 70, 90), (17000, 67, 33), (6000, 300, 130), (300, 40, 5000), (3, 17, 65536)]
 ACTS = [("none", 1.0), ("relu", 1.0), ("silu", 1.0), ("gelu", 1.0), ("softplus", 100.0), ("sine", 30.0)]
 
 
@@ -280,7 +280,7 @@ def test_rows_beyond_32_bits(gpu_ash):
 @pytest.mark.parametrize("out_dtype", TYPES, ids=ids)
 @pytest.mark.parametrize("shape", [(1, 16, 1), (1, 1024, 64), (7, 3, 5), (16, 131, 33), (40, 600, 48), (65, 128, 64),
                                    (130, 67, 129), (1000, 257, 300), (16500, 400, 1008), (2500, 272, 1000),
-                                   (9000, 2064, 136)], ids=str)
+                                   (9000, 2064, 136), (9000, 300, 20), (4000, 131, 200), (17000, 67, 33), (300, 40, 5000)], ids=str)
 def test_linear_of_8_bit_rows(gpu_ash, shape, out_dtype):
     rows, k, m = shape
     x, w, b, r, _, _ = operands(rows, k, m, torch.float32, seed=11)

@@ -116,6 +116,11 @@ __device__ inline Values<T, N> read(const T* p, int64_t left) {
     }
     return r;
 }
+template <typename T, int N> __device__ inline Values<T, N> read(const T* p) {
+    Values<T, N> r;
+    __builtin_memcpy(&r, p, sizeof(r));
+    return r;
+}
 
 // ---------------------------------------------------------------- three bf16 numbers
 struct Three {
@@ -1298,12 +1303,13 @@ __global__ __launch_bounds__((Tile<SIZE, SIZE>::kThreads), 2) void large_kernel(
     }
 }
 
-// Few rows: 16 columns for 16 rows a workgroup, whose eight wavefronts share out k and
-// join their sums in LDS.  Operands go from memory straight into the matrix instructions:
-// every value of the weight is read once and used once, so there is nothing to keep.
+// Few rows: 16 columns for RB times 16 rows a workgroup, whose eight wavefronts share out k
+// and join their sums in LDS.  Operands go from memory straight into the matrix instructions:
+// a value of the weight is read once and used for the workgroup's rows, so there is nothing
+// to keep.  Sixteen rows are bound by the weight's bytes: of 4096 float32 to 4096 19.6 us
+// (67 MB, 3.4 TB/s), in bf16 9.7, in e4m3 6.2; one row of 64 by the launch, 2.3 us.
 constexpr int kFewThreads = 512;
 constexpr int kFewWaves = kFewThreads / 64;
-constexpr int kAhead = 4;   // steps whose operands are on their way at a time
 
 template <typename T> __device__ inline Fragment<T> formed(const Values<T, Form<T>::kLane>& v) {
     Fragment<T> f;
@@ -1320,47 +1326,74 @@ template <typename T> __device__ inline Fragment<T> formed(const Values<T, Form<
     return f;
 }
 
-template <typename T, typename TO>
+template <typename T, typename TO, int RB>
 __global__ __launch_bounds__(kFewThreads) void few_rows_kernel(const Product a) {
     constexpr int kEach = Form<T>::kLane * 4;   // values of k a step
-    __shared__ float sums[kFewWaves][16][20];
+    constexpr int kAhead = RB == 1 ? 4 : 2;     // steps whose operands are on their way at a time
+    __shared__ float sums[kFewWaves][RB * 16][20];
     const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), g = lane >> 4;
-    const int64_t col0 = static_cast<int64_t>(blockIdx.x) * 16, row0 = static_cast<int64_t>(blockIdx.y) * 16;
+    const int64_t col0 = static_cast<int64_t>(blockIdx.x) * 16, row0 = static_cast<int64_t>(blockIdx.y) * RB * 16;
     const int64_t row = row0 + (lane & 15), col = col0 + (lane & 15);
-    const bool has_row = row < a.p.rows, has_col = col < a.q.rows;
-    const T* p = static_cast<const T*>(a.p.p) + (has_row ? row : 0) * a.p.stride;
-    const T* q = static_cast<const T*>(a.q.p) + (has_col ? col : 0) * a.q.stride;
-    f32x4 acc = {0.0f, 0.0f, 0.0f, 0.0f};
-    for (int64_t k0 = static_cast<int64_t>(wave) * kEach; k0 < a.k; k0 += kAhead * kFewWaves * kEach) {
-        Fragment<T> fp[kAhead], fq[kAhead];
+    // (what rows and columns beyond the last ones get is not written: they take the first's)
+    const T* p[RB];
+#pragma unroll
+    for (int r = 0; r < RB; ++r) p[r] = static_cast<const T*>(a.p.p) + (row + r * 16 < a.p.rows ? row + r * 16 : 0) * a.p.stride;
+    const T* q = static_cast<const T*>(a.q.p) + (col < a.q.rows ? col : 0) * a.q.stride;
+    f32x4 acc[RB] = {};
+    int64_t k0 = static_cast<int64_t>(wave) * kEach;
+    for (; k0 + (kAhead - 1) * kFewWaves * kEach + kEach <= a.k; k0 += kAhead * kFewWaves * kEach) {
+        Values<T, Form<T>::kLane> vp[kAhead][RB], vq[kAhead];
 #pragma unroll
         for (int i = 0; i < kAhead; ++i) {
             const int64_t k = k0 + i * kFewWaves * kEach + g * Form<T>::kLane;
-            fq[i] = formed<T>(read<T, Form<T>::kLane>(q + k, has_col ? a.k - k : 0));
-            fp[i] = formed<T>(read<T, Form<T>::kLane>(p + k, has_row ? a.k - k : 0));
+            vq[i] = read<T, Form<T>::kLane>(q + k);
+#pragma unroll
+            for (int r = 0; r < RB; ++r) vp[i][r] = read<T, Form<T>::kLane>(p[r] + k);
         }
 #pragma unroll
-        for (int i = 0; i < kAhead; ++i) acc = mma(fq[i], fp[i], acc);
-    }
-    *reinterpret_cast<f32x4*>(&sums[wave][lane & 15][g * 4]) = acc;
-    __syncthreads();
-    if (threadIdx.x >= 256) return;
-    const int r = threadIdx.x >> 4, c = threadIdx.x & 15;
-    const int64_t out_row = row0 + r, out_col = col0 + c;
-    if (out_row >= a.p.rows || out_col >= a.q.rows) return;
-    float z[1] = {0.0f}, y[1], d[1];
+        for (int i = 0; i < kAhead; ++i) {
+            const Fragment<T> fq = formed<T>(vq[i]);
 #pragma unroll
-    for (int i = 0; i < kFewWaves; ++i) z[0] += sums[i][r][c];
+            for (int r = 0; r < RB; ++r) acc[r] = mma(fq, formed<T>(vp[i][r]), acc[r]);
+        }
+    }
+    for (; k0 + kEach <= a.k; k0 += kFewWaves * kEach) {
+        const int64_t k = k0 + g * Form<T>::kLane;
+        const Values<T, Form<T>::kLane> vq = read<T, Form<T>::kLane>(q + k);
+        Values<T, Form<T>::kLane> vp[RB];
+#pragma unroll
+        for (int r = 0; r < RB; ++r) vp[r] = read<T, Form<T>::kLane>(p[r] + k);
+        const Fragment<T> fq = formed<T>(vq);
+#pragma unroll
+        for (int r = 0; r < RB; ++r) acc[r] = mma(fq, formed<T>(vp[r]), acc[r]);
+    }
+    if (k0 < a.k) {   // at most one step of one wavefront
+        const int64_t k = k0 + g * Form<T>::kLane;
+        const Fragment<T> fq = formed<T>(read<T, Form<T>::kLane>(q + k, a.k - k));
+#pragma unroll
+        for (int r = 0; r < RB; ++r) acc[r] = mma(fq, formed<T>(read<T, Form<T>::kLane>(p[r] + k, a.k - k)), acc[r]);
+    }
+#pragma unroll
+    for (int r = 0; r < RB; ++r) *reinterpret_cast<f32x4*>(&sums[wave][r * 16 + (lane & 15)][g * 4]) = acc[r];
+    __syncthreads();
     const LinearJob& j = a.job;
-    if constexpr (Form<T>::kScaled) z[0] *= j.input_scales[out_row] * j.weight_scales[out_col];
-    if (j.bias != nullptr) z[0] += as_float(static_cast<const TO*>(j.bias)[out_col]);
-    activate<sizeof(TO) == 4>(j.activation, j.act_scale, z, y, d);
-    if (j.residual != nullptr) y[0] += as_float(static_cast<const TO*>(j.residual)[out_row * j.residual_stride + out_col]);
-    const int64_t o = out_row * a.q.rows + out_col;
-    static_cast<TO*>(j.out)[o] = static_cast<TO>(y[0]);
-    if (j.slope_out != nullptr) {
-        using Slope = typename Form<TO>::Slope;
-        static_cast<Slope*>(j.slope_out)[o] = static_cast<Slope>(d[0]);
+    for (int at = threadIdx.x; at < RB * 256; at += kFewThreads) {
+        const int r = at >> 4, c = at & 15;
+        const int64_t out_row = row0 + r, out_col = col0 + c;
+        if (out_row >= a.p.rows || out_col >= a.q.rows) continue;
+        float z[1] = {0.0f}, y[1], d[1];
+#pragma unroll
+        for (int i = 0; i < kFewWaves; ++i) z[0] += sums[i][r][c];
+        if constexpr (Form<T>::kScaled) z[0] *= j.input_scales[out_row] * j.weight_scales[out_col];
+        if (j.bias != nullptr) z[0] += as_float(static_cast<const TO*>(j.bias)[out_col]);
+        activate<sizeof(TO) == 4>(j.activation, j.act_scale, z, y, d);
+        if (j.residual != nullptr) y[0] += as_float(static_cast<const TO*>(j.residual)[out_row * j.residual_stride + out_col]);
+        const int64_t o = out_row * a.q.rows + out_col;
+        static_cast<TO*>(j.out)[o] = static_cast<TO>(y[0]);
+        if (j.slope_out != nullptr) {
+            using Slope = typename Form<TO>::Slope;
+            static_cast<Slope*>(j.slope_out)[o] = static_cast<Slope>(d[0]);
+        }
     }
 }
 
@@ -1700,7 +1733,20 @@ __global__ __launch_bounds__(kJoinThreads) void join_kernel(const float* parts, 
 }
 
 // ------------------------------------------------------------------------ launches
-constexpr int64_t kFewRows = 64;
+// Workgroups of few_rows_kernel, of eight wavefronts each, up to which it is taken: two for
+// every CU, which run at once (twice as many of 32 rows in types whose products cost more
+// than their bytes).  us of the tiles and of few rows, to both sides of the rule:
+//   rows x in x out        float32       bf16         e4m3 to bf16
+//     64 x 256 x 256       10.1   3.4    5.8   2.7     5.4   2.6
+//    512 x 256 x 256       10.1   4.1    5.9   3.2     5.4   2.9
+//     16 x 4096 x 4096      126  19.6   61.4   9.7    44.4   6.2
+//     64 x 4096 x 4096      107  46.7   43.0  23.5    19.8  13.4
+//    256 x 1024 x 1024     29.4  14.2   12.9   7.8     8.3   5.2
+//    512 x 1024 x 1024     29.5  25.1   13.1  13.2     8.4   8.4 (beyond it)
+//   1024 x 1024 x 1024     30.2  46.7   13.3  23.7     8.7  14.3 (beyond it for all)
+//   2048 x 64 x 64          6.5   3.1    3.7   2.7     8.0   4.3
+//   8192 x 64 x 64          6.8   5.5    3.8   3.6     8.1   8.0 (beyond it)
+constexpr int64_t kFewGroups = 512;
 
 int64_t tiles_of(int64_t n, int size) { return (n + size - 1) / size; }
 int power_of(int64_t n) {   // the next power of two, up to 64
@@ -1783,6 +1829,13 @@ template <typename T> int join(const LinearJob& j, int64_t parts, int64_t bias_f
     return 0;
 }
 
+template <typename T, typename TO, int RB> int launch_few(const Product& a, hipStream_t s) {
+    few_rows_kernel<T, TO, RB><<<dim3(static_cast<unsigned>(tiles_of(a.q.rows, 16)),
+                                      static_cast<unsigned>(tiles_of(a.p.rows, RB * 16))), kFewThreads, 0, s>>>(a);
+    ASH_LAUNCH_CHECK();
+    return 0;
+}
+
 template <typename T> int launch_narrow_backward(const Product& a, hipStream_t s) {
     const unsigned grid = static_cast<unsigned>(narrow_backward_parts(a.k, a.pairs));
     const bool m = a.job.cols > 32, k = a.q.rows > 32;
@@ -1797,13 +1850,9 @@ template <typename T> int launch_narrow_backward(const Product& a, hipStream_t s
 template <typename T, typename TO, int KIND>
 int launch_by_size(const Product& a, hipStream_t s) {
     if constexpr (KIND == kLinearForward) {
-        if (a.p.rows <= kFewRows) {
-            few_rows_kernel<T, TO><<<dim3(static_cast<unsigned>(tiles_of(a.q.rows, 16)),
-                                          static_cast<unsigned>(tiles_of(a.p.rows, 16))),
-                                     kFewThreads, 0, s>>>(a);
-            ASH_LAUNCH_CHECK();
-            return 0;
-        }
+        const int64_t across = tiles_of(a.q.rows, 16);
+        if (a.p.rows <= 16 || across * tiles_of(a.p.rows, 16) <= kFewGroups) return launch_few<T, TO, 1>(a, s);
+        if (across * tiles_of(a.p.rows, 32) <= (sizeof(T) == 1 ? kFewGroups : 2 * kFewGroups)) return launch_few<T, TO, 2>(a, s);
     }
     if constexpr (KIND != kLinearGradWeight) {
         const int ks = power_of(tiles_of(a.k, 4 * Form<T>::kLane)), kc = power_of(tiles_of(a.q.rows, 16));
