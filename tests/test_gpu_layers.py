@@ -276,6 +276,83 @@ def test_rows_beyond_32_bits(gpu_ash):
     assert torch.equal(q.scales[-300:], small.scales)
 
 
+def test_wide_rows_beyond_32_bits(gpu_ash):
+    """More than 2^31 values in every operand of the large tiles."""
+    rows, k, m, few = 525_000, 4104, 4112, 90
+    g = torch.Generator().manual_seed(30)
+    at = torch.cat([torch.arange(few // 2), torch.arange(rows - few // 2, rows)]).to(DEV)
+    part, up, w = (rand(g, few, k, dtype=torch.bfloat16), rand(g, few, m, dtype=torch.bfloat16),
+                   rand(g, m, k, size=k**-0.5, dtype=torch.bfloat16))
+    x = torch.zeros(rows, k, dtype=torch.bfloat16, device=DEV)
+    x[at] = part
+    gy = torch.zeros(rows, m, dtype=torch.bfloat16, device=DEV)
+    gy[at] = up
+    lx, lw = leaves(x, w)
+    out = gpu_ash.linear(lx, lw, activation="silu")
+    y, d, _, _ = ref.linear(part, w, None, "silu")
+    ref.check(out[at], y, torch.bfloat16)
+    assert int(out.any(1).sum()) == few
+    gx, gw = torch.autograd.grad(out, [lx, lw], gy)
+    want = ref.linear_gradients(up, part, w, d, "silu", torch.bfloat16)
+    ref.check(gx[at], want[0], torch.bfloat16)
+    ref.check(gw, want[1], torch.bfloat16)
+    assert int(gx.any(1).sum()) == few
+
+
+def test_rows_beyond_one_grid(gpu_ash):
+    """More workgroups than a grid holds threads for."""
+    rows = (1 << 30) + 77
+    x = torch.full((rows, 1), 3.0, dtype=torch.bfloat16, device=DEV)
+    x[-5:] = -2.0
+    out = gpu_ash.rms_norm(x, eps=7.0)
+    assert bool((out[:-5] == 0.75).all()) and bool((out[-5:] == torch.tensor(-2 / 11**0.5).bfloat16().to(DEV)).all())
+    lx, = leaves(x)
+    gx, = torch.autograd.grad(gpu_ash.rms_norm(lx, eps=7.0), lx, torch.ones_like(x))
+    assert bool((gx[:-5] == torch.tensor(7 / 64).bfloat16().to(DEV)).all())
+    assert bool((gx[-5:] == torch.tensor(7 / 11**1.5).bfloat16().to(DEV)).all())
+
+
+def test_the_largest_layer(gpu_ash):
+    """65536 features in and out: a weight of 2^32 values."""
+    n, rows = 65536, 3
+    g = torch.Generator().manual_seed(31)
+    w = torch.zeros(n, n, dtype=torch.bfloat16, device=DEV)
+    at = torch.tensor([0, 1, 777, n // 2 - 1, n // 2, n - 2, n - 1], device=DEV)
+    w[at] = rand(g, len(at), n, size=n**-0.5, dtype=torch.bfloat16)
+    x, gy = rand(g, rows, n, dtype=torch.bfloat16), rand(g, rows, n, dtype=torch.bfloat16)
+    lx, lw = leaves(x, w)
+    out = gpu_ash.linear(lx, lw)
+    y, d, _, _ = ref.linear(x, w[at], None)
+    ref.check(out[:, at], y, torch.bfloat16)
+    gx, gw = torch.autograd.grad(out, [lx, lw], gy)
+    want = ref.linear_gradients(gy[:, at], x, w[at], d, "none", torch.bfloat16)
+    ref.check(gx, want[0], torch.bfloat16)
+    ref.check(gw[at], want[1], torch.bfloat16)
+    assert bool((gw.view(-1, 8, n)[:, 5, :9] == (gy.double().t() @ x.double()[:, :9]).bfloat16().view(-1, 8, 9)[:, 5]).all())
+
+
+@pytest.mark.parametrize("rows", [3, 20, 40, 700, 30000])
+@pytest.mark.parametrize("dtype", TYPES, ids=ids)
+def test_what_is_not_finite_in_the_first_row_stays_there(gpu_ash, rows, dtype):
+    """Rows and columns beyond the last ones of a tile may be made of the first."""
+    x, w, b, _, gy, _ = operands(rows, 70, 40, dtype, seed=32)
+    lx, lw, lb = leaves(x, w, b)
+    plain = gpu_ash.linear(lx, lw, lb, activation="gelu")
+    gx = torch.autograd.grad(plain, lx, gy)[0]
+    x, w, b, gy = x.clone(), w.clone(), b.clone(), gy.clone()
+    x[0, 0], w[0, 1], b[0], gy[0, 2] = float("nan"), float("nan"), float("inf"), float("nan")
+    lx, = leaves(x)
+    out = gpu_ash.linear(lx, w, b, activation="gelu")
+    assert out[0].isnan().all() and out[:, 0].isnan().all()
+    assert torch.equal(out[1:, 1:], plain[1:, 1:])
+    w[0, 1] = 0.5   # a finite weight again: the other rows' gradients
+    lx, = leaves(x)
+    out = gpu_ash.linear(lx, w, None, activation="none")
+    clean = torch.autograd.grad(gpu_ash.linear(lx, w, None), lx, torch.nan_to_num(gy))[0]
+    got, = torch.autograd.grad(out, lx, gy)
+    assert got[0].isnan().all() and torch.equal(got[1:], clean[1:]) and gx.isfinite().all()
+
+
 # --------------------------------------------------------------------- 8-bit rows
 @pytest.mark.parametrize("out_dtype", TYPES, ids=ids)
 @pytest.mark.parametrize("shape", [(1, 16, 1), (1, 1024, 64), (7, 3, 5), (16, 131, 33), (40, 600, 48), (65, 128, 64),
@@ -559,6 +636,24 @@ def test_a_capture_beside_an_eager_graph_of_the_same_leaves_is_refused(gpu_ash):
     del kept
     out = gpu_ash.linear(x, w)
     assert torch.autograd.grad(out.sum(), x)[0].shape == x.shape
+
+
+def test_a_broadcast_residual_with_a_gradient_is_not_captured(gpu_ash):
+    x, w, r = torch.randn(40, 8, device=DEV), torch.randn(8, 8, device=DEV), torch.randn(8, device=DEV)
+    lr, = leaves(r)
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    for call in (lambda: gpu_ash.linear(x, w, residual=lr), lambda: gpu_ash.rms_norm(x, residual=lr)):
+        with torch.cuda.stream(side):
+            graph = torch.cuda.CUDAGraph()
+            graph.capture_begin()
+            with pytest.raises(RuntimeError, match="broadcast residual"):
+                call()
+            kept = gpu_ash.linear(x, w, residual=r)
+            graph.capture_end()
+        torch.cuda.synchronize()
+        del kept
+    assert torch.autograd.grad(gpu_ash.linear(x, w, residual=lr).sum(), lr)[0].tolist() == [40.0] * 8
 
 
 def test_third_order_is_refused(gpu_ash):

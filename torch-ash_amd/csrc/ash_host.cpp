@@ -1174,6 +1174,14 @@ void leaves_may_be_captured(std::initializer_list<const Tensor*> tensors) {
     }
 }
 
+// The gradient of a broadcast residual is summed by torch, whose sums clear memory by a
+// node that replays of a graph do not repeat reliably.
+void may_broadcast(const Optional& residual, const Optional& rows) {
+    if (!residual.has_value() || !residual->requires_grad() || residual->numel() == rows->numel()) return;
+    need(c10::hip::currentStreamCaptureStatusMayInitCtx() == c10::hip::CaptureStatus::None,
+         "the gradient of a broadcast residual may not be captured: give the residual the output's shape");
+}
+
 // The gradients of a dense layer as a node of their own, so that they have gradients too.
 // Tensors that are not there are not arguments of a node (torch numbers its edges by those
 // that are), hence the optionals, and it returns the gradients that are asked for only.
@@ -1374,6 +1382,7 @@ Tensor linear(const Tensor& x, const Tensor& w, const Optional& b, const std::st
     const bool learns = at::GradMode::is_enabled() &&
                         (x.requires_grad() || w.requires_grad() || (b.has_value() && b->requires_grad()) ||
                          (r.has_value() && r->requires_grad()));
+    if (learns) may_broadcast(residual, r);
     if (learns) leaves_may_be_captured({&x, &w, b.has_value() ? &*b : &x, residual.has_value() ? &*residual : &x});
     const Tensor out = learns ? Linear::apply(rows, w, b, r, f.kind, f.scale)
                               : linear_forward(readable(rows), w.contiguous(), b.has_value() ? b->contiguous() : Tensor(),
@@ -1621,6 +1630,7 @@ std::tuple<Tensor, Optional, Optional> rms_norm(const Tensor& x, const Optional&
     const auto back = [&](const Tensor& t) { return x.dim() == 2 ? t : t.reshape(shape); };
     if (learns) {
         need(!quantize, "rms_norm: 8-bit rows have no gradients; call it under torch.no_grad()");
+        may_broadcast(residual, r);
         leaves_may_be_captured({&x, w.has_value() ? &*w : &x, residual.has_value() ? &*residual : &x});
         const variable_list out = Norm::apply(rows, w, r, eps);
         return {back(out[0]), out.size() > 1 ? Optional(back(out[1])) : std::nullopt, std::nullopt};

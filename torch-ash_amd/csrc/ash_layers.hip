@@ -103,7 +103,12 @@ __device__ inline void join(float (&v)[N], float (*space)[N]) {
 struct NormDev {
     ash_norm_args a;
     float inverse_cols;
+    int64_t first;   // forward: row of the launch's first workgroup
 };
+
+// A grid holds fewer than 2^32 threads: longer work takes several launches of this many
+// workgroups.
+constexpr int64_t kMaxGroups = 1 << 23;
 
 // Where a thread stands: row of the workgroup's, lane of the row's, first value of chunk i.
 template <int kLanes> struct Lane {
@@ -118,7 +123,7 @@ __global__ __launch_bounds__(kThreads) void norm_forward_kernel(const NormDev d)
     const Lane<kLanes> me;
     const ash_norm_args& a = d.a;
     __shared__ float space[kThreads / 64][1];
-    const int64_t row = static_cast<int64_t>(blockIdx.x) * Lane<kLanes>::kRows + me.row;
+    const int64_t row = d.first + static_cast<int64_t>(blockIdx.x) * Lane<kLanes>::kRows + me.row;
     const bool there = row < a.rows;
     if (kLanes <= 64 && !there) return;
     float s[kChunks][8];
@@ -401,10 +406,16 @@ int64_t parts_of(int64_t rows, int64_t cols) {
 enum NormKind { kNormForward, kNormBackward, kNormSecond };
 
 template <typename T, int kLanes, int kChunks>
-int launch_norm(NormKind kind, const NormDev& d, hipStream_t s) {
-    const int64_t each = kThreads / kLanes, groups = (d.a.rows + each - 1) / each;
+int launch_norm(NormKind kind, NormDev d, hipStream_t s) {
     if (kind == kNormForward) {
-        norm_forward_kernel<T, kLanes, kChunks><<<static_cast<unsigned>(groups), kThreads, 0, s>>>(d);
+        constexpr int64_t kEach = kThreads / kLanes;
+        for (; d.first < d.a.rows; d.first += kMaxGroups * kEach) {
+            const int64_t groups = (d.a.rows - d.first + kEach - 1) / kEach;
+            norm_forward_kernel<T, kLanes, kChunks>
+                    <<<static_cast<unsigned>(groups < kMaxGroups ? groups : kMaxGroups), kThreads, 0, s>>>(d);
+            ASH_LAUNCH_CHECK();
+        }
+        return 0;
     } else {
         const unsigned grid = static_cast<unsigned>(parts_of(d.a.rows, d.a.cols));
         if (kind == kNormBackward) norm_backward_kernel<T, kLanes, kChunks><<<grid, kThreads, 0, s>>>(d);
@@ -463,7 +474,7 @@ int run_norm(NormKind kind, const ash_norm_args* args, void* stream, const char*
     if ((a.rows > 1 && a.input_stride < 0) || a.residual_stride < 0) ASH_FAIL(std::string(what) + ": bad strides");
     PointerGuard guard;
     ASH_HIP(guard.enter_for(a.rows > 0 ? a.input : a.weight_out));
-    const NormDev d = {a, 1.0f / static_cast<float>(a.cols)};
+    const NormDev d = {a, 1.0f / static_cast<float>(a.cols), 0};
     hipStream_t s = static_cast<hipStream_t>(stream);
     if (a.dtype == ASH_F32) return norm_of<float>(kind, d, s);
     if (a.dtype == ASH_BF16) return norm_of<__bf16>(kind, d, s);
@@ -476,13 +487,15 @@ constexpr int64_t kMaxFeatures = 65536;
 // grad * slope, rounded to the operands' type as the products round it.
 template <typename T, typename S>
 __global__ __launch_bounds__(kThreads) void scale_kernel(const T* grad, const S* slope, float factor, T* out, int64_t n) {
-    const int64_t at = (static_cast<int64_t>(blockIdx.x) * kThreads + threadIdx.x) * 8;
-    float g[8], d[8];
-    read8(grad + at, n - at, g);
-    read8(slope + at, n - at, d);
+    const int64_t step = static_cast<int64_t>(gridDim.x) * kThreads * 8;
+    for (int64_t at = (static_cast<int64_t>(blockIdx.x) * kThreads + threadIdx.x) * 8; at < n; at += step) {
+        float g[8], d[8];
+        read8(grad + at, n - at, g);
+        read8(slope + at, n - at, d);
 #pragma unroll
-    for (int i = 0; i < 8; ++i) g[i] *= factor * d[i];
-    write8(out + at, n - at, g);
+        for (int i = 0; i < 8; ++i) g[i] *= factor * d[i];
+        write8(out + at, n - at, g);
+    }
 }
 
 int run_linear(LinearKind kind, const LinearJob& j, int32_t dtype, hipStream_t s) {
@@ -613,12 +626,11 @@ int ash_linear_scale_gradient(const ash_linear_args* args, const void* grad, con
     if (args->rows == 0) return 0;
     if (grad == nullptr || slope == nullptr || scaled == nullptr) ASH_FAIL("null pointer in linear_scale_gradient");
     const int64_t n = args->rows * args->out_features, groups = (n + kThreads * 8 - 1) / (kThreads * 8);
-    if (groups > 0x7FFFFFFFll) ASH_FAIL("linear_scale_gradient: too many rows");
     const float factor = job_of(*args).slope_factor;
     PointerGuard guard;
     ASH_HIP(guard.enter_for(grad));
     hipStream_t s = static_cast<hipStream_t>(stream);
-    const unsigned grid = static_cast<unsigned>(groups);
+    const unsigned grid = static_cast<unsigned>(groups < kMaxGroups ? groups : kMaxGroups);
     if (args->dtype == ASH_F32) {
         scale_kernel<<<grid, kThreads, 0, s>>>(static_cast<const float*>(grad), static_cast<const float*>(slope), factor,
                                                static_cast<float*>(scaled), n);

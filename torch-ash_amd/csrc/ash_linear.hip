@@ -1761,7 +1761,7 @@ int launch(Product a, hipStream_t s) {
     a.col_tiles = tiles_of(a.q.rows, BC);
     const int64_t tiles = a.row_tiles * a.col_tiles * (KIND == kLinearGradWeight ? a.parts * a.pairs : 1);
     const int64_t groups = (tiles + kXcds - 1) / kXcds * kXcds;
-    if (groups > 0x7FFFFFFFll) ASH_FAIL("linear: too many rows");
+    if (groups * Tile<BR, BC>::kThreads > 0xFFFFFFFFll) ASH_FAIL("linear: too many rows");   // HIP's limit of a grid
     product_kernel<T, TO, BR, BC, KIND><<<static_cast<unsigned>(groups), Tile<BR, BC>::kThreads, 0, s>>>(a);
     ASH_LAUNCH_CHECK();
     return 0;
@@ -1780,7 +1780,7 @@ int launch_large(Product a, hipStream_t s) {
     a.col_tiles = tiles_of(a.q.rows, SIZE);
     const int64_t tiles = a.row_tiles * a.col_tiles * (KIND == kLinearGradWeight ? a.parts * a.pairs : 1);
     const int64_t groups = (tiles + kXcds - 1) / kXcds * kXcds;
-    if (groups > 0x7FFFFFFFll) ASH_FAIL("linear: too many rows");
+    if (groups * Tile<SIZE, SIZE>::kThreads > 0xFFFFFFFFll) ASH_FAIL("linear: too many rows");
     large_kernel<T, TO, SIZE, KIND><<<static_cast<unsigned>(groups), Tile<SIZE, SIZE>::kThreads, 0, s>>>(a);
     ASH_LAUNCH_CHECK();
     return 0;
@@ -1821,9 +1821,10 @@ template <typename T> int join(const LinearJob& j, int64_t parts, int64_t bias_f
     join_kernel<T, n><<<static_cast<unsigned>(tiles_of(values, n) + tiles_of(j.cols, n)), kJoinThreads, 0, s>>>( \
             static_cast<const float*>(j.scratch), values, j.cols, parts, bias_first, bias_parts,                 \
             static_cast<T*>(j.weight_out), static_cast<T*>(j.bias_out))
-    // 32 threads for a value's parts where there are many (narrow layers), or eight
+    // 32 threads for a value's parts where there are many (narrow layers), eight, or one
     if (parts > 64) ASH_JOIN(32);
-    else ASH_JOIN(128);
+    else if (parts > 4) ASH_JOIN(128);
+    else ASH_JOIN(1024);
 #undef ASH_JOIN
     ASH_LAUNCH_CHECK();
     return 0;
