@@ -122,3 +122,43 @@ def test_the_c_abi_refuses_missing_buffers():
     assert lib.ash_norm_backward(ctypes.byref(n), None) == 1
     assert "scratch" in lib.ash_last_error().decode()
     assert lib.ash_norm_forward(None, None) == 1
+
+
+def test_the_c_abi_refuses_what_the_narrow_and_the_scaled_gradients_do_not_take():
+    lib = common.load_library()
+    a = linear_args(lib)
+    both = lambda a, grad=4096, gx=4096, gw=4096, scratch=4096, size=1 << 30, second=(None, None, None), stride=0: \
+        lib.ash_linear_backward_both(ctypes.byref(a), grad, None, *second, stride, gx, gw, None, scratch, size, None)
+    assert lib.ash_linear_backward_both_scratch_bytes(2, 3, 4, 0, 1) >= (3 * 4 + 4) * 4
+    for sizes in ((0, 3, 4, 0, 1), (2, 65, 4, 0, 1), (2, 3, 65, 0, 1), (2, 3, 4, 4, 1), (2, 3, 4, 0, 0), (-1, 3, 4, 0, 1)):
+        assert lib.ash_linear_backward_both_scratch_bytes(*sizes) == 0
+    for bad in (dict(grad=None), dict(gx=None), dict(gw=None), dict(scratch=None), dict(size=8),
+                dict(second=(4096, None, None)), dict(second=(4096, None, 4096), stride=-1)):
+        assert both(a, **bad) == 1, bad
+    for changes in (dict(in_features=65), dict(out_features=65), dict(rows=0), dict(dtype=4, out_dtype=0), dict(rows=-1)):
+        assert both(linear_args(lib, **changes)) == 1, changes
+    # what the output tells of the slope: of float32, of two activations
+    for dtype, activation in ((0, 2), (0, 0), (0, 5), (2, 1), (3, 4)):
+        assert not lib.ash_linear_slope_by_output(dtype, activation)
+        bent = linear_args(lib, dtype=dtype, out_dtype=dtype, activation=activation, slope_is_output=1)
+        assert lib.ash_linear_backward_input(ctypes.byref(bent), 4096, 4096, None, 4096, None) == 1
+        assert "slope" in lib.ash_last_error().decode()
+    assert lib.ash_linear_slope_by_output(0, 1) and lib.ash_linear_slope_by_output(0, 4)
+    assert not lib.ash_linear_wants_scaled_gradient(1 << 20, 1024, 1024, 0)
+    for missing in range(3):
+        buffers = [None if i == missing else 4096 for i in range(3)]
+        assert lib.ash_linear_scale_gradient(ctypes.byref(a), *buffers, None) == 1
+    assert lib.ash_linear_scale_gradient(None, 4096, 4096, 4096, None) == 1
+
+
+def test_the_c_abi_refuses_strides_of_the_second_order():
+    lib = common.load_library()
+    a = linear_args(lib)
+    assert lib.ash_linear_second(ctypes.byref(a), 4096, 4096, -1, None, 0, 4096, None, None) == 1
+    assert lib.ash_linear_second(ctypes.byref(a), 4096, 4096, 3, 4096, -1, 4096, None, None) == 1
+    assert lib.ash_linear_second(ctypes.byref(a), 4096, 4096, 3, None, 0, None, None, None) == 1
+    assert lib.ash_linear_second(ctypes.byref(linear_args(lib, input_stride=-1)), 4096, 4096, 3, None, 0, 4096, None, None) == 1
+    for call in (lib.ash_norm_backward, lib.ash_norm_second):
+        n = common._NormArgs(input=4096, output=4096, rows=2, cols=3, input_stride=3, normalise=1)
+        assert call(ctypes.byref(n), None) == 1   # no grad
+        assert call(None, None) == 1
