@@ -145,6 +145,8 @@ def test_the_c_abi_refuses_what_the_narrow_and_the_scaled_gradients_do_not_take(
         assert "slope" in lib.ash_last_error().decode()
     assert lib.ash_linear_slope_by_output(0, 1) and lib.ash_linear_slope_by_output(0, 4)
     assert not lib.ash_linear_wants_scaled_gradient(1 << 20, 1024, 1024, 0)
+    told = linear_args(lib, activation=1, slope_is_output=1)
+    assert lib.ash_linear_scale_gradient(ctypes.byref(told), 4096, 4096, 4096, None) == 1
     for missing in range(3):
         buffers = [None if i == missing else 4096 for i in range(3)]
         assert lib.ash_linear_scale_gradient(ctypes.byref(a), *buffers, None) == 1

@@ -1205,9 +1205,11 @@ struct LinearGrad : torch::autograd::Function<LinearGrad> {
                 return out;
             }
         }
-        if (need_x) out.push_back(linear_backward_input(grad, d, w, Tensor(), f));
+        Tensor gz = grad, left = d;
+        if (need_w) scale_gradient(gz, left, x, w, f);
+        if (need_x) out.push_back(linear_backward_input(gz, left, w, Tensor(), f));
         if (need_w || need_b) {
-            auto [gw, gb] = linear_backward_weight({grad, d, x}, {}, false, need_w, need_b, f);
+            auto [gw, gb] = linear_backward_weight({gz, left, x}, {}, false, need_w, need_b, f);
             if (need_w) out.push_back(gw);
             if (need_b) out.push_back(gb);
         }
@@ -1253,13 +1255,15 @@ struct LinearGrad : torch::autograd::Function<LinearGrad> {
                 return out;
             }
         }
+        Tensor gz = grad, left = d;
+        if (need_w && u.defined()) scale_gradient(gz, left, x, w, f);
         if (need_x) {
-            if (of_w.defined()) out[1] = linear_backward_input(grad, d, of_w, Tensor(), f);
+            if (of_w.defined()) out[1] = linear_backward_input(gz, left, of_w, Tensor(), f);
             if (q.defined()) out[1] = linear_backward_input(q, Tensor(), w, out[1], f);
             if (!out[1].defined()) out[1] = at::zeros_like(x);
         }
         if (need_w || need_b) {
-            const Pair first{grad, d, u}, second{q, Tensor(), x};
+            const Pair first{gz, left, u}, second{q, Tensor(), x};
             std::pair<Tensor, Tensor> of{Tensor(), Tensor()};
             const bool has_bias = need_b && q.defined();
             if (u.defined() && need_w) of = linear_backward_weight(first, q.defined() ? second : Pair{}, has_bias, true, has_bias, f);
@@ -1319,8 +1323,8 @@ struct Linear : torch::autograd::Function<Linear> {
                 for (int i = 0; i < 3; ++i) out[i] = (*all)[i];
                 return out;
             }
-            scale_gradient(grad, d, x, w, f);
         }
+        if (need_w) scale_gradient(grad, d, x, w, f);
         if (need_x) out[0] = linear_backward_input(grad, d, w.contiguous(), Tensor(), f);
         if (need_w || need_b) {
             std::tie(out[1], out[2]) = linear_backward_weight({grad, d, readable(x)}, {}, false, need_w, need_b, f);

@@ -1868,15 +1868,14 @@ int launch_by_size(const Product& a, hipStream_t s) {
         if (t.cols == 32) return launch<T, TO, 128, 32, KIND>(a, s);
         if (t.rows == 64) return launch<T, TO, 64, 64, KIND>(a, s);
         if constexpr (Form<T>::kParts == 1) {
-            if (t.cols >= 128) {
-                if (takes_large<T>(a.p, a.p.rows) && takes_large<T>(a.q, a.q.rows) &&
-                    (a.pairs == 1 || (takes_large<T>(a.p2, a.p.rows) && takes_large<T>(a.q2, a.q.rows)))) {
-                    return t.cols == 256 ? launch_large<T, TO, 256, KIND>(a, s) : launch_large<T, TO, 128, KIND>(a, s);
-                }
-                return launch<T, TO, 128, 128, KIND>(a, s);
+            if (t.cols >= 128 && takes_large<T>(a.p, a.p.rows) && takes_large<T>(a.q, a.q.rows) &&
+                (a.pairs == 1 || (takes_large<T>(a.p2, a.p.rows) && takes_large<T>(a.q2, a.q.rows)))) {
+                return t.cols == 256 ? launch_large<T, TO, 256, KIND>(a, s) : launch_large<T, TO, 128, KIND>(a, s);
             }
+            return launch<T, TO, 64, 64, KIND>(a, s);
+        } else {
+            return launch<T, TO, 128, 64, KIND>(a, s);
         }
-        return launch<T, TO, 128, 64, KIND>(a, s);
     }
     if (a.q.rows <= 32) return launch<T, TO, 128, 32, KIND>(a, s);
     if constexpr (Form<T>::kParts == 1 && KIND != kLinearSecond && !std::is_same<T, WideE4M3>::value) {
@@ -1887,11 +1886,27 @@ int launch_by_size(const Product& a, hipStream_t s) {
             if (tiles_of(a.p.rows, 128) * tiles_of(a.q.rows, 128) >= 128) return launch_large<T, TO, 128, KIND>(a, s);
         }
     }
-    if (tiles_of(a.p.rows, 128) * tiles_of(a.q.rows, 64) < 256) return launch<T, TO, 64, 64, KIND>(a, s);
-    if constexpr (Form<T>::kParts == 1) {
-        if (a.q.rows > 64) return launch<T, TO, 128, 128, KIND>(a, s);
+    // Tiles of 64 x 64 keep most workgroups under way and waste least (us of 64 x 64, 128 x 64,
+    // 128 x 128; 10 007 rows of 131 fp16 to 257: 13.6 15.2 19.3, its gradient of the input 14.1
+    // 18.9 21.8; 10 007 rows of 512 fp32 to 512: 54 62, the gradient 73 98; 40 000 rows of 333
+    // e4m3 to 515: 56 53 62).  Larger ones read less where there are many: in 16 bits from two
+    // a CU on, unless the last one is mostly nothing (65 536 rows of 256, gradient of the
+    // input: 58 72 44; 40 000 of 131 to 257 forward 55 52 46), of the second order, which keeps
+    // twice as much a row, from sixteen of the small ones (65 536 rows of 256: 67 59 63; 5000
+    // of 131 to 257 11.7 12.7 16.0), and in float32 from eight with long k, but not of the
+    // gradient of the input, whose turning loads take more registers (65 536 rows of 512:
+    // forward 291 278, second 512 492, gradient 363 390; second of 10 007 of 2048 to 256, below
+    // the rule, 161 201).
+    const int64_t row_tiles = tiles_of(a.p.rows, KIND == kLinearSecond ? 32 : 64), tiles = row_tiles * tiles_of(a.q.rows, 64);
+    if constexpr (KIND == kLinearSecond || (KIND == kLinearForward && Form<T>::kIsFloat)) {
+        if (Form<T>::kIsFloat ? tiles >= 2048 && a.k >= 512 : tiles >= 4096) return launch<T, TO, 128, 64, KIND>(a, s);
+    } else if constexpr (!Form<T>::kIsFloat && !Form<T>::kScaled) {
+        const int64_t across = tiles_of(a.q.rows, 128);
+        if (tiles_of(a.p.rows, 128) * across >= 512 && across * 8 <= tiles_of(a.q.rows, 64) * 5) {
+            return launch<T, TO, 128, 128, KIND>(a, s);
+        }
     }
-    return launch<T, TO, 128, 64, KIND>(a, s);
+    return launch<T, TO, 64, 64, KIND>(a, s);
 }
 
 }  // namespace
