@@ -1400,8 +1400,10 @@ __global__ __launch_bounds__(kFewThreads) void few_rows_kernel(const Product a) 
 // Narrow layers: the weight's fragments stay in registers, and every wavefront takes sixteen
 // rows after sixteen rows through them, straight from memory (a lane's operand of an
 // instruction is 16 or 32 consecutive bytes of a row; the next rows are on their way while
-// these are multiplied).  No barriers, LDS only on the way out.  Bound by memory: 524 288 rows
-// of 64 float32 to 64, of softplus.
+// these are multiplied).  No barriers, LDS only on the way out.  524 288 rows of 64 float32
+// to 64 take 53 us without an activation (268 MB, 5.1 TB/s: bound by memory) and 73 with
+// softplus, whose arithmetic (half of it transcendental or in twice the precision) adds to
+// that at two wavefronts a SIMD; two steps of rows on their way instead of one: 79.
 // KS: steps of k (4 kLane values each), KC: times sixteen columns.
 constexpr int kNarrowThreads = 256;
 template <typename T, typename TO, int KS, int KC, int KIND>
@@ -1799,8 +1801,11 @@ template <typename T> constexpr bool narrow_fits(int kind, int ks, int kc) {
 template <typename T, typename TO, int KIND, int KS, int KC> int launch_narrow(const Product& a, hipStream_t s) {
     if constexpr (narrow_fits<T>(KIND, KS, KC)) {
         const int64_t groups = tiles_of(a.p.rows, kNarrowThreads / 64 * 16);
-        // as many workgroups as are under way at once
-        const int64_t most = KIND != kLinearSecond && narrow_registers<T>(KS, KC) <= 12 ? 1024 : 512;
+        // as many workgroups as are under way at once, two a CU or, with fewer registers, three
+        // (524 288 rows of 32 float32 to 64: 48 us for 50 forward, 52 for 72 the gradient of the
+        // input, 74 for 93 the second order; four a CU 72 and 92; 64 to 64, whose workgroups are
+        // two a CU, 98 us forward by two and 104 by three)
+        const int64_t most = narrow_registers<T>(KS, KC) <= 12 ? 768 : 512;
         narrow_kernel<T, TO, KS, KC, KIND><<<static_cast<unsigned>(groups < most ? groups : most), kNarrowThreads, 0, s>>>(a);
         ASH_LAUNCH_CHECK();
     }
