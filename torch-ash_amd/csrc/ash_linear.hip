@@ -493,22 +493,42 @@ __device__ inline f32x4 sum_rows(const Fragment<float>& p, f32x4 c) {
 // --------------------------------------------------------------------- activations
 template <bool FULL> __device__ inline float sigmoid(float v) { return __builtin_amdgcn_rcpf(1.0f + exp_of<FULL>(-v)); }
 
-// The normal distribution's integral and its density at z.  The complementary error function
-// is t exp(-x^2 + P(t)), t = 1 / (1 + x / 2), with the Chebyshev fit erfcc of Press et al.,
-// Numerical Recipes (1.2e-7 of the value, everywhere).
+// The normal distribution's integral and its density at z, with e = exp(-z^2 / 2), x = |z| /
+// sqrt(2).  FULL: the complementary error function is t exp(-x^2 + P(t)), t = 1 / (1 + x / 2),
+// with the Chebyshev fit erfcc of Press et al., Numerical Recipes (1.2e-7 of the value,
+// everywhere).  For results of 16 bits e t P(t), t = 1 / (1 + 0.46 x), P fitted to erfc(x)
+// exp(x^2) / t such that the largest relative error is least, 2^-19.9 of the value everywhere:
+// one exponential less (65 536 rows of 1024 bf16 to 1024 forward, of which the activation's
+// arithmetic is a sixth: 183 us for 201).
 template <bool FULL> __device__ inline void normal(float z, float& integral, float& density) {
-    const float x = fabsf(z) * 0.70710678f, t = __builtin_amdgcn_rcpf(fmaf(0.5f, x, 1.0f));
-    float p = 0.17087277f;
-    p = fmaf(p, t, -0.82215223f);
-    p = fmaf(p, t, 1.48851587f);
-    p = fmaf(p, t, -1.13520398f);
-    p = fmaf(p, t, 0.27886807f);
-    p = fmaf(p, t, -0.18628806f);
-    p = fmaf(p, t, 0.09678418f);
-    p = fmaf(p, t, 0.37409196f);
-    p = fmaf(p, t, 1.00002368f);
-    p = fmaf(p, t, -1.26551223f);
-    const float e = exp_of<FULL>(-0.5f * z * z), tail = 0.5f * t * e * exp_of<FULL>(p);
+    float e, tail;
+    if constexpr (FULL) {
+        const float x = fabsf(z) * 0.70710678f, t = __builtin_amdgcn_rcpf(fmaf(0.5f, x, 1.0f));
+        float p = 0.17087277f;
+        p = fmaf(p, t, -0.82215223f);
+        p = fmaf(p, t, 1.48851587f);
+        p = fmaf(p, t, -1.13520398f);
+        p = fmaf(p, t, 0.27886807f);
+        p = fmaf(p, t, -0.18628806f);
+        p = fmaf(p, t, 0.09678418f);
+        p = fmaf(p, t, 0.37409196f);
+        p = fmaf(p, t, 1.00002368f);
+        p = fmaf(p, t, -1.26551223f);
+        e = exp_of<true>(-0.5f * z * z);
+        tail = 0.5f * t * e * exp_of<true>(p);
+    } else {
+        const float t = __builtin_amdgcn_rcpf(fmaf(0.32526913f, fabsf(z), 1.0f));
+        float p = 0.033857174f;   // P / 2
+        p = fmaf(p, t, -0.11331463f);
+        p = fmaf(p, t, 0.084595464f);
+        p = fmaf(p, t, 0.02630535f);
+        p = fmaf(p, t, 0.093423873f);
+        p = fmaf(p, t, 0.11559094f);
+        p = fmaf(p, t, 0.12977864f);
+        p = fmaf(p, t, 0.12976353f);
+        e = __builtin_amdgcn_exp2f(z * z * -0.72134752f);
+        tail = e * t * p;
+    }
     integral = z > 0.0f ? 1.0f - tail : tail;
     density = 0.39894228f * e;
 }
