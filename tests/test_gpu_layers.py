@@ -71,6 +71,22 @@ def test_linear_and_its_gradients_in_large_tiles(gpu_ash, rows, k, m, kind, dtyp
             ref.check(have, want, dtype, what)
 
 
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16], ids=ids)
+@pytest.mark.parametrize("rows,k,m", [(16640, 136, 1000), (4100, 136, 264), (16500, 72, 1004)])
+def test_residuals_of_large_tiles(gpu_ash, rows, k, m, dtype):
+    """Of rows that lie apart, at addresses that are not aligned, that broadcast; of
+    8-bit operands too."""
+    x, w, b, wide, _, _ = operands(rows, k, m, dtype, seed=21)
+    y, _, _, _ = ref.linear(x, w, b, "gelu", 1.0)
+    apart = torch.cat([wide, wide[:, :16]], 1)
+    q = [gpu_ash.QuantizedRows.of(t) for t in (x, w)]
+    of8, _, _, _ = ref.linear(q[0].data.float(), q[1].data.float(), b, "silu", 1.0, None, q[0].scales, q[1].scales, True)
+    for r in (wide, apart[:, 8:m + 8], apart[:, 3:m + 3], wide[:1].expand(rows, m), wide[5], wide[:, :1]):
+        more = r.expand(rows, m).double()
+        ref.check(gpu_ash.linear(x, w, b, activation="gelu", residual=r), y + ref.Off(more), dtype)
+        ref.check(gpu_ash.linear(*q, b, activation="silu", residual=r), of8 + ref.Off(more), dtype)
+
+
 @pytest.mark.parametrize("dtype", TYPES, ids=ids)
 @pytest.mark.parametrize("kind,a", ACTS)
 def test_activations(gpu_ash, kind, a, dtype):

@@ -798,7 +798,9 @@ struct Finish {
     }
     // first_row: the same for a wavefront, so that a row's address is a scalar one and the
     // lane's offset from it
-    __device__ void rows(const Product& a, const char* space, int64_t first_row) const {
+    // STAGED: the lane's 16 bytes of the residual lie at `staged` and every kilobyte from there
+    template <bool STAGED = false>
+    __device__ void rows(const Product& a, const char* space, int64_t first_row, const char* staged = nullptr) const {
         const LinearJob& j = a.job;
         const int r0 = lane / kLanes;
         const int32_t offset = r0 * static_cast<int32_t>(a.q.rows) + static_cast<int32_t>(col);
@@ -840,7 +842,12 @@ struct Finish {
                 }
             } else {
                 float more[N];
-                if (j.residual != nullptr) {
+                if constexpr (STAGED) {
+                    Values<TO, N> v;
+                    __builtin_memcpy(&v, staged + i * 1024, 16);
+#pragma unroll
+                    for (int e = 0; e < N; ++e) more[e] = as_float(v.v[e]);
+                } else if (j.residual != nullptr) {
                     get_values(static_cast<const TO*>(j.residual) + row * j.residual_stride + (r0 * j.residual_stride + col),
                                left, more);
                 }
@@ -853,7 +860,7 @@ struct Finish {
                         put_values(static_cast<Slope*>(j.slope_out) + o + offset, left, d);
                     }
                 }
-                if (j.residual != nullptr) {
+                if (STAGED || j.residual != nullptr) {
 #pragma unroll
                     for (int e = 0; e < N; ++e) y[e] += more[e];
                 }
@@ -1292,6 +1299,50 @@ struct LargeWork {
     }
 };
 
+// The way out with a residual, which comes by way of LDS (`staged`, 8 KB of the wavefront's
+// own) sixty-four rows at a time: loads into registers between the stores would wait for
+// those stores, sixteen times a tile (65 536 rows of 1024 bf16 to 1024, GELU, slopes and
+// residual: 250 us for 276).
+template <typename TO, int SIZE, bool SCALED>
+__device__ inline void finish_staged(const Product& a, char* space, char* staged,
+                                     const f32x4 (&acc)[Tile<SIZE, SIZE>::kR][Tile<SIZE, SIZE>::kC], int64_t row0,
+                                     int64_t col0) {
+    using W = Tile<SIZE, SIZE>;
+    using Out = Finish<TO, W::kC, kLinearForward, SCALED>;
+    static_assert(sizeof(TO) == 2 && Out::kDown == 8 && W::kR % 4 == 0, "a strip of sixteen rows is two kilobytes");
+    const LinearJob& j = a.job;
+    const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), lane = threadIdx.x & 63;
+    const int64_t first_col = col0 + wave % W::kWaveCols * W::kC * 16;
+    const int64_t first_row = row0 + wave / W::kWaveCols * W::kR * 16;
+    Out out;
+    out.start(a, first_col);
+    const uint32_t step = static_cast<uint32_t>(j.residual_stride) * 2;
+    const char* base = static_cast<const char*>(j.residual) + (first_row * j.residual_stride + first_col) * 2;
+    const auto buffer = __builtin_amdgcn_make_buffer_rsrc(const_cast<char*>(base), 0, 0x7FFFFFFF, 0x00020000);
+#pragma unroll 1
+    for (int quad = 0; quad < W::kR / 4; ++quad) {
+#pragma unroll
+        for (int i = 0; i < 8; ++i) {
+            const int row = quad * 64 + i * 8 + lane / 8;
+            const bool there = first_row + row < a.p.rows && out.left > 0;
+            __builtin_amdgcn_raw_ptr_buffer_load_lds(
+                    buffer, (__attribute__((address_space(3))) void*)(staged + i * 1024), 16,
+                    there ? row * step + lane % 8 * 16 : kNowhere, 0, 0, 0);
+        }
+        __builtin_amdgcn_s_waitcnt(kWaitAll);
+        asm volatile("" ::: "memory");
+#pragma unroll 1
+        for (int n = 0; n < 4; ++n) {
+#pragma unroll
+            for (int now = 0; now < W::kR; ++now) {
+                if (now == quad * 4 + n) out.give(space, acc[now]);
+            }
+            out.template rows<true>(a, space, first_row + (quad * 4 + n) * 16, staged + n * 2048 + lane * 16);
+        }
+        asm volatile("" ::: "memory");
+    }
+}
+
 template <typename T, typename TO, int SIZE, int KIND>
 __global__ __launch_bounds__((Tile<SIZE, SIZE>::kThreads), 2) void large_kernel(const Product a) {
     constexpr bool kStackP = KIND == kLinearGradWeight, kStackQ = KIND != kLinearForward;
@@ -1319,6 +1370,18 @@ __global__ __launch_bounds__((Tile<SIZE, SIZE>::kThreads), 2) void large_kernel(
         work.template run<false>({p0, q0}, {p1, q1}, {p2, q2}, {p3, q3});
         __syncthreads();   // of all wavefronts' reads of their operands
         char* space = (work.wave < kHalf ? p0 : q0) + work.wave % kHalf * W::kOutBytes;
+        if constexpr (KIND == kLinearForward && sizeof(TO) == 2) {
+            const LinearJob& j = a.job;
+            if (j.residual != nullptr && reinterpret_cast<uintptr_t>(j.residual) % 16 == 0 && j.residual_stride % 8 == 0 &&
+                j.residual_stride < (1 << 21) && a.q.rows % 8 == 0) {
+                constexpr int kEach = kFour ? W::kWaves / 4 : W::kWaves / 2;   // wavefronts a plane
+                static_assert(kEach * 8192 <= Work::kP, "");
+                const int of = work.wave / kEach;
+                char* plane = kFour ? (of == 0 ? p1 : of == 1 ? p2 : of == 2 ? q1 : q2) : (of == 0 ? p1 : q1);
+                finish_staged<TO, SIZE, Form<T>::kScaled>(a, space, plane + work.wave % kEach * 8192, work.acc, row0, col0);
+                return;
+            }
+        }
         finish<TO, SIZE, SIZE, KIND, Form<T>::kScaled>(a, space, work.acc, row0, col0);
     }
 }
