@@ -1994,7 +1994,7 @@ int launch_by_size(const Product& a, hipStream_t s) {
     const int64_t row_tiles = tiles_of(a.p.rows, KIND == kLinearSecond ? 32 : 64), tiles = row_tiles * tiles_of(a.q.rows, 64);
     if constexpr (KIND == kLinearSecond || (KIND == kLinearForward && Form<T>::kIsFloat)) {
         if (Form<T>::kIsFloat ? tiles >= 2048 && a.k >= 512 : tiles >= 4096) return launch<T, TO, 128, 64, KIND>(a, s);
-    } else if constexpr (!Form<T>::kIsFloat && !Form<T>::kScaled) {
+    } else if constexpr (KIND != kLinearGradWeight && !Form<T>::kIsFloat && !Form<T>::kScaled) {
         const int64_t across = tiles_of(a.q.rows, 128);
         if (tiles_of(a.p.rows, 128) * across >= 512 && across * 8 <= tiles_of(a.q.rows, 64) * 5) {
             return launch<T, TO, 128, 128, KIND>(a, s);
