@@ -1879,7 +1879,8 @@ template <typename T> constexpr int narrow_registers(int ks, int kc) {
     return ks * kc * Form<T>::kParts * (Form<T>::kIsByte ? 2 : 1);
 }
 template <typename T> constexpr bool narrow_fits(int kind, int ks, int kc) {
-    return narrow_registers<T>(ks, kc) <= (kind != kLinearForward && ks == 4 ? 16 : 32) && (!Form<T>::kScaled || ks * kc < 16 || (ks < 4 && Form<T>::kIsByte));
+    return narrow_registers<T>(ks, kc) <= (kind != kLinearForward && ks == 4 ? 16 : 32) &&
+           (!Form<T>::kScaled || ks * kc < 16 || (ks < 4 && Form<T>::kIsByte));
 }
 
 template <typename T, typename TO, int KIND, int KS, int KC> int launch_narrow(const Product& a, hipStream_t s) {
@@ -1910,7 +1911,9 @@ template <typename T> int join(const LinearJob& j, int64_t parts, int64_t bias_f
     join_kernel<T, n><<<static_cast<unsigned>(tiles_of(values, n) + tiles_of(j.cols, n)), kJoinThreads, 0, s>>>( \
             static_cast<const float*>(j.scratch), values, j.cols, parts, bias_first, bias_parts,                 \
             static_cast<T*>(j.weight_out), static_cast<T*>(j.bias_out))
-    // 32 threads for a value's parts where there are many (narrow layers), eight, or one
+    // 32 threads for a value's parts where there are many (narrow layers: 65 536 rows of 32 bf16
+    // to 128 14.8 us with the product, by eight 17.1), eight, or one (8192 rows of 4096 to 4096
+    // 270 us with the product, by eight 310, and a grid holds weights of 2^32 values so)
     if (parts > 64) ASH_JOIN(32);
     else if (parts > 4) ASH_JOIN(128);
     else ASH_JOIN(1024);
