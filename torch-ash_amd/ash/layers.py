@@ -74,8 +74,11 @@ def linear(
 
     Gradients of first and second order exist for every operand (of the gradient
     of a weight too, not of third order).  For them the forward keeps the slope of
-    the activation at every output, in float32 (float16 for bfloat16 operands).  They are the same
-    numbers on every run.
+    the activation at every output, in float32 (float16 for bfloat16 operands), or,
+    for float32 relu and softplus without a residual, the output itself, which must
+    not be changed in place before the backward pass then.  They are the same
+    numbers on every run.  While a graph is captured, a broadcast residual that
+    needs a gradient is refused, and so are leaves that an eager graph still holds.
 
     With 8-bit rows (`QuantizedRows`, both or neither) every sum of products is
     multiplied by the scales of its two rows; bias and residual have the type of
@@ -109,7 +112,8 @@ def rms_norm(
     Returns the normed rows, or with a residual (normed rows, s).  With `quantize`
     the normed rows are `QuantizedRows`, rounded to 8 bits from float32 by the
     same kernel (no gradients then).  Gradients of first and second order exist
-    for every operand."""
+    for every operand.  Squares are float32: a row of values beyond 1e19 gives
+    zeros."""
     _must_stand_alone("rms_norm", input, weight, residual)
     normed, total, scales = core.backend.host.rms_norm(input, weight, residual, eps, quantize)
     if quantize:
